@@ -240,7 +240,7 @@ def _prepare_clip(case, rand):
     if not own:
         out = {t: torch.zeros_like(flat[t]) for t in kinds}
         return dict(state, grads=cut(flat), cuts=cut(out), out=out)
-    from cubecl_amd import ElemType, Mi355Runtime, TensorHandle
+    from cubecl_amd import ElemType, Mi355Runtime, TensorHandle, ops
     client = Mi355Runtime.client()
     torch.cuda.synchronize()
     h = {t: (client.empty(ends[t] * size_of(t)), client.empty(ends[t] * size_of(t))) for t in kinds}
@@ -248,7 +248,7 @@ def _prepare_clip(case, rand):
     [(views[t][0].copy_(flat[t]), views[t][1].zero_()) for t in kinds]
     handles = [[TensorHandle.new_contiguous(shape, h[t][side].offset_start_by(at * size_of(t)), _elem(t)) for shape, t, at in slots] for side in (0, 1)]
     total = client.empty(4)
-    return dict(state, client=client, grads=handles[0], cuts=handles[1], out={t: views[t][1] for t in kinds},
+    return dict(state, client=client, grads=ops.TensorList(handles[0]), cuts=ops.TensorList(handles[1]), out={t: views[t][1] for t in kinds},
                 total=TensorHandle.new_contiguous((1,), total, ElemType.F32), total_view=_view(total, (1,), "f32"))
 
 

@@ -52,6 +52,7 @@ ATOMIC_USAGE = {"LoadStore": 1, "Exchange": 2, "Add": 4, "MinMax": 8, "Bitwise":
 ADDRESS_TYPE_U32, ADDRESS_TYPE_U64 = 1, 2
 LAYOUT_ROW_MAJOR, LAYOUT_COL_MAJOR = 0, 1
 
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 REDUCE_SUM, REDUCE_MEAN, REDUCE_MAX, REDUCE_MIN, REDUCE_PROD, REDUCE_ARGMAX, REDUCE_ARGMIN = 0, 1, 2, 3, 4, 5, 6
 PLANE_PROD, PLANE_INCLUSIVE_SUM, PLANE_EXCLUSIVE_SUM, PLANE_INCLUSIVE_PROD, PLANE_EXCLUSIVE_PROD = 100, 101, 102, 103, 104
 (PLANE_ALL, PLANE_ANY, PLANE_ELECT, PLANE_BROADCAST, PLANE_SHUFFLE, PLANE_SHUFFLE_XOR, PLANE_SHUFFLE_UP, PLANE_SHUFFLE_DOWN,
@@ -141,6 +142,58 @@ class GemmScaledDesc(C.Structure):
                [(n, C.c_int32) for n in ("dtype_a", "dtype_b", "dtype_c", "block", "algo", "reserved")]
 
 
+class GemmEpilogue(C.Structure):
+    """mi355_gemm_epilogue."""
+    _fields_ = [
+        ("bias", C.c_void_p), ("residual", C.c_void_p),
+        ("pre", C.c_void_p),
+        ("row_scale", C.c_void_p), ("col_scale", C.c_void_p),
+        ("stride_bias", C.c_int64),
+        ("ld_residual", C.c_int64), ("stride_residual", C.c_int64),
+        ("ld_pre", C.c_int64), ("stride_pre", C.c_int64),
+        ("inc_row_scale", C.c_int64), ("stride_row_scale", C.c_int64), ("inc_col_scale", C.c_int64), ("stride_col_scale", C.c_int64),
+        ("activation", C.c_int32), ("dtype_bias", C.c_int32),
+    ]
+
+
+class GemmFusedGradDesc(C.Structure):
+    """mi355_gemm_fused_grad_desc."""
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int64), ("batch", C.c_int64),
+        ("ld_out", C.c_int64), ("ld_pre", C.c_int64), ("ld_grad", C.c_int64),
+        ("stride_out", C.c_int64), ("stride_pre", C.c_int64), ("stride_grad", C.c_int64),
+        ("dtype", C.c_int32), ("activation", C.c_int32), ("dtype_bias", C.c_int32), ("batch_bias", C.c_int32),
+    ]
+
+
+class RmsNormDesc(C.Structure):
+    """mi355_rms_norm_desc."""
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("ld_in", C.c_int64), ("ld_residual", C.c_int64), ("ld_hidden", C.c_int64), ("ld_out", C.c_int64), ("ld_scales", C.c_int64),
+        ("eps", C.c_float),
+        ("dtype", C.c_int32), ("dtype_weight", C.c_int32), ("dtype_out", C.c_int32), ("scale_block", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class RmsNormGradDesc(C.Structure):
+    """mi355_rms_norm_grad_desc."""
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("ld_out", C.c_int64), ("ld_hidden", C.c_int64), ("ld_in", C.c_int64), ("ld_stream", C.c_int64),
+        ("dtype", C.c_int32), ("dtype_weight", C.c_int32), ("dtype_grad_weight", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class TensorSpan(C.Structure):
+    """mi355_tensor_span."""
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("rows", C.c_uint64), ("cols", C.c_uint64), ("row_stride", C.c_uint64),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 MAX_RANK = 8
 COPY_PATH_FLAT, COPY_PATH_ROWS, COPY_PATH_TRANSPOSE, COPY_PATH_GENERIC, COPY_PATH_TWO_SIDED = range(5)
 
@@ -217,6 +270,16 @@ PROTOTYPES = {
     "mi355_cast": (C.c_int32, [_P, _P, _P, C.c_int32, _P, C.c_int32, C.c_uint64]),
     "mi355_gemm": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), _P, _P, _P]),
     "mi355_gemm_add": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), _P, _P, _P, _P]),
+    "mi355_gemm_fused": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), C.POINTER(GemmEpilogue), _P, _P, _P]),
+    "mi355_gemm_fused_plan": (C.c_int32, [C.POINTER(GemmDesc), _I32P]),
+    "mi355_gemm_fused_grad_workspace_bytes": (C.c_int32, [C.POINTER(GemmFusedGradDesc), _U64P]),
+    "mi355_gemm_fused_grad": (C.c_int32, [_P, _P, C.POINTER(GemmFusedGradDesc), _P, _P, _P, _P, _P, C.c_uint64]),
+    "mi355_rms_norm": (C.c_int32, [_P, _P, C.POINTER(RmsNormDesc), _P, _P, _P, _P, _P, _P, _P]),
+    "mi355_rms_norm_grad_workspace_bytes": (C.c_int32, [C.POINTER(RmsNormGradDesc), _U64P]),
+    "mi355_rms_norm_grad": (C.c_int32, [_P, _P, C.POINTER(RmsNormGradDesc), _P, _P, _P, _P, _P, _P, _P, _P, C.c_uint64]),
+    "mi355_global_norm_workspace_bytes": (C.c_int32, [_U64P]),
+    "mi355_global_norm": (C.c_int32, [_P, _P, C.POINTER(TensorSpan), C.c_uint32, _P, _P, C.c_uint64]),
+    "mi355_clip_by_global_norm": (C.c_int32, [_P, _P, C.POINTER(TensorSpan), C.POINTER(TensorSpan), C.c_uint32, C.c_float, _P, _P, C.c_uint64]),
     "mi355_gemm_select": (C.c_int32, [_P, C.POINTER(GemmDesc), _I32P]),
     "mi355_gemm_tail_plan": (C.c_int32, [C.POINTER(GemmDesc), _I32P, C.POINTER(C.c_int64), _I32P]),
     "mi355_gemm_split_plan": (C.c_int32, [C.POINTER(GemmDesc), C.c_int32, _I32P]),

@@ -1,5 +1,6 @@
 // gemm.cpp -- mi355_gemm: descriptor validation and kernel selection.
 #include "gemm_common.hpp"
+#include "linear_ops.hpp"
 
 using namespace mi355;
 
@@ -846,6 +847,45 @@ MI355_API int32_t mi355_gemm_add(mi355_ctx *ctx, mi355_stream stream, const mi35
     if (rc != MI355_OK) return rc;
     launch_add_c(s, static_cast<const float *>(prod), c, d_out, d.batch, d.m, d.n, d.dtype_c, d.ldc, d.stride_c);
     check_launch(ctx, "mi355_gemm_add");
+    return MI355_OK;
+}
+
+// act(rs cs (A B) + bias) + residual: the selected kernel writes the f32 product into library-owned per-stream scratch, gemm_epilogue.hip
+// does the rest in one pass and rounds once.
+MI355_API int32_t mi355_gemm_fused(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const mi355_gemm_epilogue *epilogue, const void *a,
+                                   const void *b, void *c)
+{
+    MI355_REQUIRE_CTX(ctx);
+    if (!epilogue) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: the epilogue is NULL");
+    int32_t rc = validate(ctx, desc, a, b, c);
+    if (rc != -1) return rc;
+    const mi355_gemm_desc &d = *desc;
+    const mi355_gemm_epilogue &ep = *epilogue;
+    rc = validate_epilogue(ctx, d, ep, a, b, c);
+    if (rc != MI355_OK) return rc;
+    hipStream_t s = stream_of(ctx, stream);
+    void *prod = nullptr;
+    const size_t bytes = (size_t)d.batch * (size_t)d.m * (size_t)d.n * sizeof(float);
+    if (scratch_get(ctx, s, SCRATCH_PRODUCT, bytes, &prod) != MI355_OK)
+        return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm_fused: no scratch for the %zu-byte f32 product (inside a capture window?)", bytes);
+    mi355_gemm_desc pd = d;
+    pd.dtype_c = MI355_DTYPE_F32;
+    pd.ldc = d.n;
+    pd.stride_c = d.m * d.n;
+    // (named kernels that hold a finished 16-bit tile: the same tile without that)
+    if (d.algo == MI355_GEMM_ALGO_LP_256Q) pd.algo = MI355_GEMM_ALGO_LP_256W4;
+    if (d.algo == MI355_GEMM_ALGO_LP_256QM) pd.algo = MI355_GEMM_ALGO_LP_256M16;
+    rc = mi355_gemm(ctx, stream, &pd, a, b, prod);
+    if (rc != MI355_OK) return rc;
+    launch_epilogue(s, static_cast<const float *>(prod), ep, c, d.batch, d.m, d.n, d.dtype_c, d.ldc, d.stride_c);
+    check_launch(ctx, "mi355_gemm_fused");
+    return MI355_OK;
+}
+
+MI355_API int32_t mi355_gemm_fused_plan(const mi355_gemm_desc *desc, int32_t *out_fused)
+{
+    if (!desc || !out_fused) return MI355_E_INVALID_ARGUMENT;
+    *out_fused = 0;
     return MI355_OK;
 }
 

@@ -1,0 +1,115 @@
+// linear_ops.hpp -- what linear_ops.cpp (argument checks, sizes, launch order) and the kernels' files share.
+#pragma once
+
+#include <algorithm>
+
+#include "internal.hpp"
+
+namespace mi355 {
+
+// ---- rms_norm.hip
+enum { OUT_PLAIN = 0, OUT_ROW = 1, OUT_BLOCK = 2 };
+
+struct norm_args {
+    const void *in, *residual, *weight;
+    void *hidden, *out, *scales;
+    float *rstd;
+    int64_t rows, cols, ld_in, ld_residual, ld_hidden, ld_out, ld_scales;
+    float eps, inv_cols;
+    int32_t dtype_weight, dtype_out;
+};
+struct norm_grad_args {
+    const void *grad_out, *hidden, *weight, *grad_hidden;
+    const float *rstd;
+    void *grad_in;
+    float *partial;           // [workgroups x rows a workgroup holds at once][cols], NULL: no weight gradient
+    int64_t rows, cols, ld_out, ld_hidden, ld_in, ld_stream;
+    float inv_cols;
+    int32_t dtype_weight;
+};
+
+// Threads and pieces for rows of `cols` elements (0 threads: the looping kernels).  Few rows leave most of the chip idle, and then
+// the row's own latency is what is waited for: as many threads as hold it in one piece.
+struct row_shape { int threads, pieces; };
+inline row_shape shape_for(int64_t rows, int64_t cols)
+{
+    if (cols > 16384) return {0, 0};
+    if (cols <= 512) return {64, 1};
+    const bool few = rows <= 512;
+    if (cols <= 1024 && !few) return {64, 2};
+    if (cols <= 2048) return {256, 1};
+    if (few && cols <= 8192) return {1024, 1};
+    if (cols <= 4096) return {256, 2};
+    if (cols <= 8192) return {256, 4};
+    return {1024, 2};
+}
+
+// workgroups of the gradient: each walks rows / grid of them and leaves one partial row (four, T = 64) of the weight's gradient
+constexpr int64_t GRAD_WGS = 512, LONG_SLABS = 64;
+inline int64_t norm_grad_wgs(int64_t rows, const row_shape &sh)
+{
+    return std::min(sh.threads == 64 ? (rows + 3) / 4 : rows, sh.threads == 1024 ? GRAD_WGS / 2 : GRAD_WGS);
+}
+inline int64_t norm_grad_partials(int64_t rows, int64_t cols)
+{
+    const row_shape sh = shape_for(rows, cols);
+    if (sh.threads == 0) return std::min(rows, LONG_SLABS);
+    return norm_grad_wgs(rows, sh) * (sh.threads == 64 ? 4 : 1);
+}
+
+void launch_rms_norm(hipStream_t s, int32_t dtype, int mode, const norm_args &a);
+void launch_rms_norm_grad(hipStream_t s, int32_t dtype, const norm_grad_args &a);
+// column sums of f32 partial rows, [batch][count][cols] -> out [batch][cols] in `dtype`; count 0: zeros
+void launch_fold_columns(hipStream_t s, const float *partial, int64_t count, int64_t cols, int64_t batch, void *out, int32_t dtype);
+
+// ---- gemm_epilogue.hip
+// what mi355_gemm_fused refuses of an epilogue (linear_ops.cpp); `d` has been validated and is not empty
+int32_t validate_epilogue(mi355_ctx *ctx, const mi355_gemm_desc &d, const mi355_gemm_epilogue &ep, const void *a, const void *b, const void *c);
+void launch_epilogue(hipStream_t s, const float *prod, const mi355_gemm_epilogue &ep, void *c, int64_t batch, int64_t m, int64_t n, int32_t dtype_c,
+                     int64_t ldc, int64_t stride_c);
+struct fused_grad_args {
+    const void *grad_out, *pre;
+    void *grad_pre;
+    float *partial;
+    int64_t m, n, batch, slab;
+    int64_t ld_out, ld_pre, ld_grad, stride_out, stride_pre, stride_grad;
+};
+void launch_fused_grad(hipStream_t s, int32_t dtype, int32_t activation, const fused_grad_args &a);
+
+// ---- global_norm.hip
+constexpr int64_t CHUNK = 16384;               // elements: 32 KiB of 16-bit, 64 KiB of f32 values
+constexpr uint32_t GRID = 1024;                // workgroups of a launch at most
+constexpr uint32_t MAX_PARTIALS = 4096;        // partial sums the workspace holds
+constexpr int FLAT_MAX = 112, ROWS_MAX = 56;
+
+struct flat_span {                             // one contiguous tensor
+    const void *in;
+    void *out;
+    int64_t n;
+    uint32_t first;                            // its first chunk in the launch's sequence
+    int32_t dtype;
+};
+struct rows_span {                             // rows of `cols` elements; a chunk is `rows_per` of them
+    const void *in;
+    void *out;
+    int64_t rows, cols, ld_in, ld_out;
+    uint32_t first;
+    int32_t dtype;
+};
+struct flat_table { uint32_t count, chunks; flat_span t[FLAT_MAX]; };
+struct rows_table { uint32_t count, chunks; rows_span t[ROWS_MAX]; };
+static_assert(sizeof(flat_table) <= 3840 && sizeof(rows_table) <= 3840, "the tables are kernel arguments");
+
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+inline int64_t rows_per_chunk(int64_t cols) { return cols >= CHUNK ? 1 : CHUNK / cols; }
+
+// one partial sum a workgroup; the norm from `count` of them; the tensors times min(1, max_norm / norm)
+void launch_square_sums(hipStream_t s, const flat_table &t, uint32_t grid, double *partial);
+void launch_square_sums(hipStream_t s, const rows_table &t, uint32_t grid, double *partial);
+void launch_finish_norm(hipStream_t s, const double *partial, uint32_t count, float *out_norm);
+void launch_scale(hipStream_t s, const flat_table &t, uint32_t grid, const double *partial, uint32_t count, float max_norm, float *out_norm);
+void launch_scale(hipStream_t s, const rows_table &t, uint32_t grid, const double *partial, uint32_t count, float max_norm, float *out_norm);
+
+}  // namespace mi355

@@ -1,0 +1,228 @@
+// rowops.hpp -- device helpers of the row-wise operators (gemm_epilogue.hip, rms_norm.hip, global_norm.hip): eight elements of any float type
+// to and from f32, reductions over a wave and a workgroup, the activations and their derivatives.
+#pragma once
+
+#include <cfloat>
+
+#include "gemm_common.hpp"
+#include "linear_ops.hpp"
+
+namespace mi355 {
+
+// ---- eight consecutive elements ------------------------------------------------------------------------------------------------
+// One row of a tensor may start at any element: the vectors below are declared with their element's alignment, which the gfx950 memory
+// pipe serves with the same 16-byte access (it splits only where a cache line ends), so odd row lengths and offset views take this path too.
+typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_e1 __attribute__((ext_vector_type(2), aligned(1)));
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ float f16_to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+
+template <int DT> struct vec8;          // the raw registers of eight elements
+template <> struct vec8<MI355_DTYPE_F32> { u32x4 lo, hi; };
+template <> struct vec8<MI355_DTYPE_BF16> { u32x4 v; };
+template <> struct vec8<MI355_DTYPE_F16> { u32x4 v; };
+
+template <int DT> constexpr int elem_size() { return DT == MI355_DTYPE_F32 ? 4 : 2; }
+
+// elements [i, i + 8) of `p`; where only `valid` < 8 of them exist the others read as zero
+template <int DT>
+__device__ __forceinline__ vec8<DT> load8(const void *p, int64_t i, int valid)
+{
+    vec8<DT> r;
+    if constexpr (DT == MI355_DTYPE_F32) {
+        const float *q = static_cast<const float *>(p) + i;
+        if (valid >= 8) {
+            r.lo = *reinterpret_cast<const u32x4_e4 *>(q);
+            r.hi = *reinterpret_cast<const u32x4_e4 *>(q + 4);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                r.lo[e] = e < valid ? __float_as_uint(q[e]) : 0u;
+                r.hi[e] = e + 4 < valid ? __float_as_uint(q[e + 4]) : 0u;
+            }
+        }
+    } else {
+        const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+        if (valid >= 8) r.v = *reinterpret_cast<const u32x4_e2 *>(q);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t lo = 2 * e < valid ? q[2 * e] : 0u, hi = 2 * e + 1 < valid ? q[2 * e + 1] : 0u;
+                r.v[e] = lo | (hi << 16);
+            }
+        }
+    }
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ float get(const vec8<DT> &r, int e)      // e a compile-time constant after unrolling
+{
+    if constexpr (DT == MI355_DTYPE_F32) return __uint_as_float(e < 4 ? r.lo[e] : r.hi[e - 4]);
+    else {
+        const uint32_t w = r.v[e >> 1];
+        if constexpr (DT == MI355_DTYPE_BF16) return __uint_as_float((e & 1) ? (w & 0xFFFF0000u) : (w << 16));
+        else return f16_to_f32((uint16_t)((e & 1) ? (w >> 16) : (w & 0xFFFFu)));
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void *p, int64_t i, int valid, const float (&f)[8])
+{
+    if constexpr (DT == MI355_DTYPE_F32) {
+        float *q = static_cast<float *>(p) + i;
+        if (valid >= 8) {
+            const u32x4 lo = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+            const u32x4 hi = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+            *reinterpret_cast<u32x4_e4 *>(q) = lo;
+            *reinterpret_cast<u32x4_e4 *>(q + 4) = hi;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < valid) q[e] = f[e];
+        }
+    } else {
+        uint16_t *q = static_cast<uint16_t *>(p) + i;
+        if (valid >= 8) {
+            const u32x4 v = {f32x2_to_lp<DT>(f[0], f[1]), f32x2_to_lp<DT>(f[2], f[3]), f32x2_to_lp<DT>(f[4], f[5]), f32x2_to_lp<DT>(f[6], f[7])};
+            *reinterpret_cast<u32x4_e2 *>(q) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < valid) q[e] = f32_to_lp<DT>(f[e]);
+        }
+    }
+}
+
+// the same with the type known at run time only (uniform over the launch)
+__device__ __forceinline__ void load8_any(const void *p, int32_t dtype, int64_t i, int valid, float (&f)[8])
+{
+    if (dtype == MI355_DTYPE_F32) {
+        const vec8<MI355_DTYPE_F32> r = load8<MI355_DTYPE_F32>(p, i, valid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = get(r, e);
+    } else if (dtype == MI355_DTYPE_BF16) {
+        const vec8<MI355_DTYPE_BF16> r = load8<MI355_DTYPE_BF16>(p, i, valid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = get(r, e);
+    } else {
+        const vec8<MI355_DTYPE_F16> r = load8<MI355_DTYPE_F16>(p, i, valid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = get(r, e);
+    }
+}
+__device__ __forceinline__ void store8_any(void *p, int32_t dtype, int64_t i, int valid, const float (&f)[8])
+{
+    if (dtype == MI355_DTYPE_F32) store8<MI355_DTYPE_F32>(p, i, valid, f);
+    else if (dtype == MI355_DTYPE_BF16) store8<MI355_DTYPE_BF16>(p, i, valid, f);
+    else store8<MI355_DTYPE_F16>(p, i, valid, f);
+}
+__device__ __forceinline__ float load1_any(const void *p, int32_t dtype, int64_t i)
+{
+    if (dtype == MI355_DTYPE_F32) return static_cast<const float *>(p)[i];
+    const uint16_t b = static_cast<const uint16_t *>(p)[i];
+    return dtype == MI355_DTYPE_BF16 ? bf16_to_f32(b) : f16_to_f32(b);
+}
+__device__ __forceinline__ void store1_any(void *p, int32_t dtype, int64_t i, float v)
+{
+    if (dtype == MI355_DTYPE_F32) static_cast<float *>(p)[i] = v;
+    else static_cast<uint16_t *>(p)[i] = dtype == MI355_DTYPE_BF16 ? f32_to_bf16_rne(v) : f32_to_f16_rne(v);
+}
+
+// ---- reductions -------------------------------------------------------------------------------------------------------------------
+// Over the 64 lanes: four DPP steps inside a row of 16 (no LDS traffic), two shuffles across the rows.  Every lane gets the result; the
+// order is fixed, so a sum is the same bits from run to run.
+template <class F, class T>
+__device__ __forceinline__ T wave_reduce(T v, F f)
+{
+    static_assert(sizeof(T) == 4, "32-bit values");
+    auto dpp = [](T x, auto ctrl) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    v = f(v, dpp(v, std::integral_constant<int, 0xB1>{}));     // quad_perm [1,0,3,2]: lane ^ 1
+    v = f(v, dpp(v, std::integral_constant<int, 0x4E>{}));     // quad_perm [2,3,0,1]: lane ^ 2
+    v = f(v, dpp(v, std::integral_constant<int, 0x141>{}));    // row_half_mirror: the other four of eight
+    v = f(v, dpp(v, std::integral_constant<int, 0x140>{}));    // row_mirror: the other eight of sixteen
+    v = f(v, __builtin_bit_cast(T, __shfl_xor(__builtin_bit_cast(int, v), 16, 64)));
+    return f(v, __builtin_bit_cast(T, __shfl_xor(__builtin_bit_cast(int, v), 32, 64)));
+}
+struct sum_of { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+// maximum of magnitudes as bit patterns: an infinity is above every number, a NaN above the infinity
+struct max_of { __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; } };
+
+// Over T threads; `slot`: T / 64 words of LDS that nobody still reads.  T == 64: each wave by itself.
+template <int T, class F, class V>
+__device__ __forceinline__ V block_reduce(V v, V *slot, F f)
+{
+    v = wave_reduce(v, f);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = slot[0];
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) v = f(v, slot[w]);
+    }
+    return v;
+}
+
+// ---- activations --------------------------------------------------------------------------------------------------------------------
+// exp through v_exp_f32 (2^x, 1 ulp): the product x * log2(e) is off by |x| 2^-24 relative, far below what 16-bit outputs show and 2^-21 of
+// the result for the |x| <= 8 that f32 outputs show.  1 / (1 + e) through v_rcp_f32 (1 ulp).
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
+// erfc(|x|) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p |x|): Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26,
+// absolute error 1.5e-7; the factor exp(-x^2) keeps the left tail of gelu free of cancellation.
+__device__ __forceinline__ float erfc_abs(float x, float exp_neg_x2)
+{
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return p * exp_neg_x2;
+}
+// z limited to [lo, hi]; a NaN stays
+__device__ __forceinline__ float limit(float z, float lo, float hi) { return z < lo ? lo : (z > hi ? hi : z); }
+
+constexpr float GELU_C0 = 0.797884560802865356f, GELU_C1 = 0.044715f;    // sqrt(2 / pi) and the cubic term of gelu's tanh form
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float z)
+{
+    if constexpr (ACT == MI355_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if constexpr (ACT == MI355_ACT_NONE) return z;
+    z = z < -FLT_MAX ? -FLT_MAX : z;                            // -inf * 0 below would be NaN where the limit is 0
+    if constexpr (ACT == MI355_ACT_SILU) return z * sigmoid_of(z);
+    if constexpr (ACT == MI355_ACT_GELU_TANH) return z * sigmoid_of(2.0f * GELU_C0 * z * (1.0f + GELU_C1 * z * z));   // (1 + tanh u) / 2 = sigmoid(2 u)
+    if constexpr (ACT == MI355_ACT_GELU) {
+        const float x = fabsf(z) * 0.707106781186547524f;
+        const float q = 0.5f * erfc_abs(x, exp_of(-x * x));
+        return z * (z < 0.0f ? q : 1.0f - q);
+    }
+    return z;
+}
+
+// The derivative.  Beyond the limits it is 0 or 1 to the last bit of f32; inside them nothing overflows.
+template <int ACT>
+__device__ __forceinline__ float act_grad_of(float z)
+{
+    if constexpr (ACT == MI355_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+    if constexpr (ACT == MI355_ACT_SILU) {
+        z = limit(z, -120.0f, 120.0f);
+        const float s = sigmoid_of(z);
+        return s * (1.0f + z * (1.0f - s));
+    }
+    if constexpr (ACT == MI355_ACT_GELU_TANH) {
+        z = limit(z, -20.0f, 20.0f);
+        const float s = sigmoid_of(2.0f * GELU_C0 * z * (1.0f + GELU_C1 * z * z));
+        return s + z * s * (1.0f - s) * (2.0f * GELU_C0) * (1.0f + 3.0f * GELU_C1 * z * z);
+    }
+    if constexpr (ACT == MI355_ACT_GELU) {
+        z = limit(z, -20.0f, 20.0f);
+        const float x = fabsf(z) * 0.707106781186547524f, ex = exp_of(-x * x);
+        const float q = 0.5f * erfc_abs(x, ex);
+        return (z < 0.0f ? q : 1.0f - q) + z * ex * 0.398942280401432678f;      // Phi(z) + z phi(z)
+    }
+    return 1.0f;
+}
+
+}  // namespace mi355

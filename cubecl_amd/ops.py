@@ -475,3 +475,486 @@ def into_contiguous_packed(client: ComputeClient, input: TensorHandle, packed_di
                                                  C.c_void_p(output.device_ptr()), C.byref(lo), logical, packed_dim, packing,
                                                  input.dtype.size()))
     return output
+
+
+# ---- a linear layer's epilogue, norms, clipping ------------------------------------------------------------------------
+_ACTIVATIONS = {"none": N.ACT_NONE, "relu": N.ACT_RELU, "gelu": N.ACT_GELU, "gelu_tanh": N.ACT_GELU_TANH, "silu": N.ACT_SILU}
+
+
+def _activation(name, what: str) -> int:
+    if name not in _ACTIVATIONS:
+        raise ServerError(N.E_UNSUPPORTED, f"{what}: unknown activation '{name}' (one of {sorted(_ACTIVATIONS)})")
+    return _ACTIVATIONS[name]
+
+
+def _ptr(t: Optional[TensorHandle]):
+    return C.c_void_p(t.device_ptr()) if t is not None else None
+
+
+def _batched(t: TensorHandle, tail: int, batch: int, what: str):
+    """(elements between batch entries, 0 for one that all entries share) of a [.., tail] operand that goes with `batch` matrices."""
+    lead = 1
+    for d in t.shape[:t.rank() - tail]:
+        lead *= d
+    if lead == 1:
+        return 0
+    if lead != batch:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: batch {lead} does not broadcast to {batch}")
+    dims = [(d, s) for d, s in zip(t.shape[:t.rank() - tail], t.strides) if d != 1]
+    for (_, s_out), (d_in, s_in) in zip(dims[:-1], dims[1:]):
+        if s_out != s_in * d_in:
+            raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: batch dims are not collapsible")
+    return dims[-1][1]
+
+
+def _vector(client: ComputeClient, t: TensorHandle, n: int, batch: int, what: str):
+    """-> (tensor, element stride, batch stride) of a per-row or per-column operand: [n] or [batch.., n], or one value for all."""
+    if t.num_elems() == 1:
+        return t, 0, 0
+    if t.shape[-1] != n:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: shape {t.shape} does not give {n} values")
+    if t.strides[-1] < 0:
+        raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: negative stride")
+    try:
+        return t, (t.strides[-1] if n > 1 else 0), _batched(t, 1, batch, what)
+    except ServerError as e:
+        if e.code != N.E_UNSUPPORTED_STRIDES:
+            raise
+    t = into_contiguous(client, t)
+    return t, (1 if n > 1 else 0), _batched(t, 1, batch, what)
+
+
+def _rows_of_matrix(t: TensorHandle, batch: int, what: str):
+    """(leading dimension, batch stride) of a row-major [.., rows, cols] tensor."""
+    rows, cols = t.shape[-2], t.shape[-1]
+    if cols > 1 and t.strides[-1] != 1:
+        raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: rows must be contiguous")
+    ld = t.strides[-2] if rows > 1 else max(cols, t.strides[-2])
+    if ld < cols:
+        raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: rows overlap")
+    return ld, _batched(t, 2, batch, what)
+
+
+def matmul_fused(client: ComputeClient, lhs: TensorHandle, rhs: TensorHandle, out: TensorHandle, *, bias: Optional[TensorHandle] = None,
+                 activation: str = "none", residual: Optional[TensorHandle] = None, lhs_scale: Optional[TensorHandle] = None,
+                 rhs_scale: Optional[TensorHandle] = None, pre_activation: Optional[TensorHandle] = None, algo: int = N.GEMM_ALGO_AUTO) -> None:
+    """out = act(lhs_scale[m] * rhs_scale[n] * (lhs @ rhs) + bias[n]) + residual: matmul with a linear layer's epilogue, formed in f32 and
+    rounded once to out's dtype (mi355_gemm_fused).
+
+    lhs, rhs and out as `matmul` takes them.  `activation`: "none" | "relu" | "gelu" | "gelu_tanh" | "silu".  `bias`: [n] or [batch.., n], f32 or
+    out's dtype.  `residual`: out's shape and dtype (any strides; may be `out` itself).  `lhs_scale` / `rhs_scale`: f32, one value, [m] / [n] or
+    [batch.., m] / [batch.., n] -- what quantising the rows of lhs and the columns of rhs to 8 bits left behind.  `pre_activation`: if given,
+    receives the activation's argument in out's shape and dtype, for matmul_fused_backward."""
+    m, k = lhs.shape[-2], lhs.shape[-1]
+    k2, n = rhs.shape[-2], rhs.shape[-1]
+    if k != k2 or out.rank() < 2 or out.shape[-2] != m or out.shape[-1] != n:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: shape mismatch {lhs.shape} x {rhs.shape} -> {out.shape}")
+    if lhs.dtype != rhs.dtype:
+        raise ServerError(N.E_INVALID_ARGUMENT, "matmul_fused: lhs/rhs dtypes differ")
+    act = _activation(activation, "matmul_fused")
+    for t, name in ((residual, "residual"), (pre_activation, "pre_activation")):
+        if t is not None and (tuple(t.shape) != tuple(out.shape) or t.dtype != out.dtype):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: {name} must have out's shape and dtype")
+    for t, name in ((lhs_scale, "lhs_scale"), (rhs_scale, "rhs_scale")):
+        if t is not None and t.dtype != ElemType.F32:
+            raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: {name} must be f32")
+    lhs, (ta, lda, ba, sa) = _kernel_ready(client, lhs, "lhs")
+    rhs, (tb, ldb, bb, sb) = _kernel_ready(client, rhs, "rhs")
+    batch = 1
+    for d in out.shape[:-2]:
+        batch *= d
+    if out.num_elems() == 0:
+        return
+    ldc, sc = _rows_of_matrix(out, batch, "matmul_fused: out")
+    for b, name in ((ba, "lhs"), (bb, "rhs")):
+        if b not in (1, batch):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: {name} batch {b} does not broadcast to {batch}")
+    ep = N.GemmEpilogue(activation=act)
+    if bias is not None:
+        bias, inc, ep.stride_bias = _vector(client, bias, n, batch, "matmul_fused: bias")
+        if inc != 1 and n > 1:                      # the kernels read it in rows of n
+            if bias.num_elems() == 1:
+                raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: bias of shape {bias.shape} does not give {n} values")
+            bias = into_contiguous(client, bias)
+            ep.stride_bias = _batched(bias, 1, batch, "matmul_fused: bias")
+        ep.bias, ep.dtype_bias = bias.device_ptr(), int(bias.dtype)
+    if residual is not None:
+        try:
+            ep.ld_residual, ep.stride_residual = _rows_of_matrix(residual, batch, "matmul_fused: residual")
+        except ServerError as e:
+            if e.code != N.E_UNSUPPORTED_STRIDES:
+                raise
+            residual = into_contiguous(client, residual)
+            ep.ld_residual, ep.stride_residual = _rows_of_matrix(residual, batch, "matmul_fused: residual")
+        ep.residual = residual.device_ptr()
+    if lhs_scale is not None:
+        lhs_scale, ep.inc_row_scale, ep.stride_row_scale = _vector(client, lhs_scale, m, batch, "matmul_fused: lhs_scale")
+        ep.row_scale = lhs_scale.device_ptr()
+    if rhs_scale is not None:
+        rhs_scale, ep.inc_col_scale, ep.stride_col_scale = _vector(client, rhs_scale, n, batch, "matmul_fused: rhs_scale")
+        ep.col_scale = rhs_scale.device_ptr()
+    if pre_activation is not None:
+        ep.ld_pre, ep.stride_pre = _rows_of_matrix(pre_activation, batch, "matmul_fused: pre_activation")
+        ep.pre = pre_activation.device_ptr()
+    desc = N.GemmDesc(m=m, n=n, k=k, batch=batch, lda=lda, ldb=ldb, ldc=ldc, stride_a=sa if ba == batch else 0, stride_b=sb if bb == batch else 0,
+                      stride_c=sc, dtype_ab=int(lhs.dtype), dtype_c=int(out.dtype), trans_a=int(ta), trans_b=int(tb), algo=algo)
+    client._s.check(client.lib.mi355_gemm_fused(
+        client.ctx, client.on(lhs, rhs, out, bias, residual, lhs_scale, rhs_scale, pre_activation), C.byref(desc), C.byref(ep),
+        C.c_void_p(lhs.device_ptr()), C.c_void_p(rhs.device_ptr()), C.c_void_p(out.device_ptr())))
+
+
+def gemm_fused_plan(client: ComputeClient, desc: N.GemmDesc) -> bool:
+    """Does mi355_gemm_fused run `desc`'s epilogue inside the product's kernel (host-side only)?"""
+    fused = C.c_int32()
+    client._s.check(client.lib.mi355_gemm_fused_plan(C.byref(desc), C.byref(fused)))
+    return bool(fused.value)
+
+
+def _swap_last(t: TensorHandle) -> TensorHandle:
+    return t.permute(tuple(range(t.rank() - 2)) + (t.rank() - 1, t.rank() - 2))
+
+
+def _as_rows(client: ComputeClient, t: TensorHandle) -> TensorHandle:
+    """[batch.., rows, cols] as one [batch * rows, cols] matrix, copied only where the batch does not follow on from the rows."""
+    if t.rank() == 2:
+        return t
+    rows, cols = 1, t.shape[-1]
+    for d in t.shape[:-1]:
+        rows *= d
+    acc, fits = t.strides[-2], True
+    for i in range(t.rank() - 3, -1, -1):
+        acc *= t.shape[i + 1]
+        fits = fits and (t.shape[i] == 1 or t.strides[i] == acc)
+    if not fits or (cols > 1 and t.strides[-1] != 1):
+        t = into_contiguous(client, t)
+    return TensorHandle.new(t.handle, (rows, cols), (max(t.strides[-2], cols), 1), t.dtype)
+
+
+def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_activation: Optional[TensorHandle], grad_pre: Optional[TensorHandle], *,
+                          activation: str = "none", grad_bias: Optional[TensorHandle] = None, lhs: Optional[TensorHandle] = None,
+                          rhs: Optional[TensorHandle] = None, grad_lhs: Optional[TensorHandle] = None, grad_rhs: Optional[TensorHandle] = None) -> None:
+    """The gradient of matmul_fused (without scales):
+
+        grad_pre = grad_out * act'(pre_activation)    grad_bias = sum of grad_pre over rows (and over a batch that shares the bias)
+        grad_lhs = grad_pre @ rhs^T                   grad_rhs = lhs^T @ grad_pre
+
+    and the residual's gradient is grad_out itself.  Outputs that are not given are not computed; grad_pre (grad_out's shape and dtype, f32, bf16
+    or f16; may be grad_out or pre_activation itself) is needed for the products, which `matmul` takes from it as it is stored; grad_bias sums it before its rounding.
+    `pre_activation` may be None for activation "none".  grad_bias: [n] or [batch.., n], f32 or grad_out's dtype.  An operand that matmul_fused
+    broadcast over the batch gets the sum over the batch."""
+    what = "matmul_fused_backward"
+    act = _activation(activation, what)
+    if grad_out.rank() < 2:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_out must have rank >= 2")
+    m, n = grad_out.shape[-2:]
+    batch = 1
+    for d in grad_out.shape[:-2]:
+        batch *= d
+    for t, name in ((pre_activation, "pre_activation"), (grad_pre, "grad_pre")):
+        if t is not None and (tuple(t.shape) != tuple(grad_out.shape) or t.dtype != grad_out.dtype):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: {name} must have grad_out's shape and dtype")
+    if pre_activation is None and act != N.ACT_NONE:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: activation '{activation}' needs pre_activation")
+    for t, of, grad, name in ((rhs, lhs, grad_lhs, "lhs"), (lhs, rhs, grad_rhs, "rhs")):
+        if grad is None:
+            continue
+        if t is None or grad_pre is None:
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_{name} needs grad_pre and the other operand")
+        if t.dtype != grad_out.dtype or grad.dtype not in (grad_out.dtype, ElemType.F32):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: the operands must have grad_out's dtype, grad_{name} that or f32")
+        if of is not None and tuple(of.shape) != tuple(grad.shape):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_{name} must have {name}'s shape")
+    if grad_lhs is not None and (grad_lhs.shape[-2] != m or rhs.shape[-1] != n or grad_lhs.shape[-1] != rhs.shape[-2]):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: shape mismatch {grad_lhs.shape} x {rhs.shape} -> {grad_out.shape}")
+    if grad_rhs is not None and (lhs.shape[-2] != m or grad_rhs.shape[-1] != n or grad_rhs.shape[-2] != lhs.shape[-1]):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: shape mismatch {lhs.shape} x {grad_rhs.shape} -> {grad_out.shape}")
+    for t, name in ((rhs if grad_lhs is not None else None, "rhs"), (lhs if grad_rhs is not None else None, "lhs"), (grad_lhs, "grad_lhs"), (grad_rhs, "grad_rhs")):
+        if t is not None and t.num_elems() // max(t.shape[-2] * t.shape[-1], 1) not in (1, batch) and t.num_elems():
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: {name} does not broadcast to batch {batch}")
+
+    def rows(t, name, writable=False):
+        try:
+            return t, _rows_of_matrix(t, batch, f"{what}: {name}")
+        except ServerError as e:
+            if writable or e.code != N.E_UNSUPPORTED_STRIDES:
+                raise
+        t = into_contiguous(client, t)
+        return t, _rows_of_matrix(t, batch, f"{what}: {name}")
+
+    desc = N.GemmFusedGradDesc(m=m, n=n, batch=batch, dtype=int(grad_out.dtype), activation=act)
+    z = None
+    if grad_out.num_elems():
+        g, (desc.ld_out, desc.stride_out) = rows(grad_out, "grad_out")
+        if act != N.ACT_NONE:
+            z, (desc.ld_pre, desc.stride_pre) = rows(pre_activation, "pre_activation")
+        if grad_pre is not None:
+            _, (desc.ld_grad, desc.stride_grad) = rows(grad_pre, "grad_pre", writable=True)
+    else:
+        g = grad_out
+    ws, need = None, C.c_uint64()
+    if grad_bias is not None:
+        if not grad_bias.is_contiguous() or grad_bias.rank() < 1 or grad_bias.shape[-1] != n:
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_bias must be contiguous, [n] or [batch.., n] (got {grad_bias.shape}, n = {n})")
+        entries = grad_bias.num_elems() // n if n else 1
+        if entries not in (1, batch):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_bias has {entries} entries for batch {batch}")
+        desc.dtype_bias, desc.batch_bias = int(grad_bias.dtype), int(entries == batch and batch > 1)
+        client._s.check(client.lib.mi355_gemm_fused_grad_workspace_bytes(C.byref(desc), C.byref(need)))
+        if need.value:
+            ws = client.empty(need.value)
+    client._s.check(client.lib.mi355_gemm_fused_grad(
+        client.ctx, client.on(g, z, grad_pre, grad_bias, ws), C.byref(desc), C.c_void_p(g.device_ptr()), _ptr(z), _ptr(grad_pre), _ptr(grad_bias),
+        _ptr(ws), need.value))
+    if grad_lhs is not None:
+        lead = grad_lhs.num_elems() // (m * grad_lhs.shape[-1]) if grad_lhs.num_elems() else batch
+        if lead == batch or grad_lhs.num_elems() == 0:
+            matmul(client, grad_pre, _swap_last(rhs), _with_batch_of(grad_lhs, grad_out))
+        else:                                       # one lhs for all entries: their sum, in f32 until the last
+            _sum_of_products(client, [(_entry(grad_pre, b), _swap_last(_entry(rhs, b))) for b in range(batch)], grad_lhs)
+    if grad_rhs is not None:
+        lead = grad_rhs.num_elems() // (n * grad_rhs.shape[-2]) if grad_rhs.num_elems() else batch
+        left_lead = lhs.num_elems() // (m * lhs.shape[-1]) if lhs.num_elems() else batch
+        if lead == batch or grad_rhs.num_elems() == 0:
+            matmul(client, _swap_last(lhs), grad_pre, _with_batch_of(grad_rhs, grad_out))
+        elif left_lead == batch:                    # one rhs for all entries: their rows under each other are one product
+            matmul(client, _swap_last(_as_rows(client, lhs)), _as_rows(client, grad_pre), _entry(grad_rhs, 0))
+        else:
+            _sum_of_products(client, [(_swap_last(_entry(lhs, b)), _entry(grad_pre, b)) for b in range(batch)], grad_rhs)
+
+
+def _with_batch_of(t: TensorHandle, model: TensorHandle) -> TensorHandle:
+    """`t` with model's rank: axes of one in front where it has fewer."""
+    extra = model.rank() - t.rank()
+    if extra <= 0:
+        return t
+    return TensorHandle.new(t.handle, (1,) * extra + tuple(t.shape), (t.shape[-2] * t.strides[-2],) * extra + tuple(t.strides), t.dtype)
+
+
+def _entry(t: TensorHandle, b: int) -> TensorHandle:
+    """Matrix `b` of a batch (the only one of a tensor that the batch shares)."""
+    offset, lead = 0, t.num_elems() // max(t.shape[-2] * t.shape[-1], 1)
+    if lead > 1:
+        for d, s in zip(reversed(t.shape[:-2]), reversed(t.strides[:-2])):
+            offset += (b % d) * s
+            b //= d
+    return TensorHandle.new(t.handle.offset_start_by(offset * t.dtype.size()), t.shape[-2:], t.strides[-2:], t.dtype)
+
+
+def _sum_of_products(client: ComputeClient, pairs, out: TensorHandle) -> None:
+    """out = sum of the products, accumulated in f32 and rounded once."""
+    out = _entry(out, 0)
+    total = TensorHandle.new_contiguous(out.shape, client.empty(out.num_elems() * 4), ElemType.F32)
+    for i, (a, b) in enumerate(pairs):
+        matmul(client, a, b, total, acc=total if i else None)
+    if out.dtype != ElemType.F32:
+        rounded = TensorHandle.new_contiguous(out.shape, client.empty(out.num_elems() * out.dtype.size()), out.dtype)
+        client._s.check(client.lib.mi355_cast(client.ctx, client.on(total, rounded), C.c_void_p(total.device_ptr()), int(ElemType.F32),
+                                              C.c_void_p(rounded.device_ptr()), int(out.dtype), out.num_elems()))
+        total = rounded
+    copy_into(client, total, out)
+
+
+def _norm_rows(t: TensorHandle, what: str):
+    """(rows, cols, row stride) of a tensor whose last axis is the norm's; E_UNSUPPORTED_STRIDES where the rows do not collapse."""
+    if t.rank() == 0:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: rank-0 tensor")
+    cols = t.shape[-1]
+    rows = 1
+    for d in t.shape[:-1]:
+        rows *= d
+    if rows == 0 or cols == 0:
+        return rows, cols, cols
+    if cols > 1 and t.strides[-1] != 1:
+        raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: last axis must have unit stride")
+    dims = [(d, s) for d, s in zip(t.shape[:-1], t.strides[:-1]) if d != 1]
+    for (_, s_out), (d_in, s_in) in zip(dims[:-1], dims[1:]):
+        if s_out != s_in * d_in:
+            raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: leading dims are not collapsible")
+    stride = dims[-1][1] if dims else cols
+    if stride < cols:
+        raise ServerError(N.E_UNSUPPORTED_STRIDES, f"{what}: rows overlap")
+    return rows, cols, stride
+
+
+def _norm_operand(client: ComputeClient, t: Optional[TensorHandle], shape, dtype, what: str):
+    """-> (operand, row stride); a view the kernels cannot walk goes through into_contiguous first."""
+    if t is None:
+        return None, 0
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: expected {tuple(shape)} {dtype.name}, got {tuple(t.shape)} {t.dtype.name}")
+    t, (_, _, stride) = _consumable(client, t, _norm_rows, what)
+    return t, stride
+
+
+def _flat(t: Optional[TensorHandle], shape, dtypes, what: str):
+    """A contiguous operand of this shape (axes of one aside) and one of these dtypes."""
+    if t is not None and ([d for d in t.shape if d != 1] != [d for d in shape if d != 1] or t.dtype not in dtypes or not t.is_contiguous()):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: expected contiguous {tuple(shape)} {'/'.join(d.name for d in dtypes)}, got {tuple(t.shape)} {t.dtype.name}")
+    return t
+
+
+_FP8 = (ElemType.F8E4M3, ElemType.F8E5M2)
+
+
+def rms_norm(client: ComputeClient, input: TensorHandle, weight: Optional[TensorHandle], output: TensorHandle, *, eps: float = 1e-6,
+             residual: Optional[TensorHandle] = None, residual_out: Optional[TensorHandle] = None, scales: Optional[TensorHandle] = None,
+             rstd: Optional[TensorHandle] = None) -> None:
+    """output = h * rstd * weight over the last axis, h = input + residual, rstd = 1 / sqrt(mean(h^2) + eps) (mi355_rms_norm).
+
+    input, residual, residual_out (receives h; may be input or residual itself): f32, bf16 or f16, one shape.  `weight`: [cols], f32 or input's
+    dtype, or None for ones.  `rstd`: f32, input's shape without the last axis (what rms_norm_backward wants).  output: input's dtype or f32; or
+    F8E4M3 / F8E5M2, and then `scales` receives one F32 per row (shape without the last axis; matmul_fused's lhs_scale) or one UE8M0 per
+    32 columns (shape [.., cols / 32]; matmul_scaled's lhs_scales), by its dtype."""
+    what = "rms_norm"
+    if input.dtype not in (ElemType.F32, ElemType.BF16, ElemType.F16):
+        raise ServerError(N.E_UNSUPPORTED, f"{what}: input must be f32, bf16 or f16")
+    if input.rank() == 0:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: rank-0 tensor")
+    shape, cols = tuple(input.shape), input.shape[-1]
+    f8 = output.dtype in _FP8
+    if tuple(output.shape) != shape:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: output has shape {tuple(output.shape)}, input {shape}")
+    if f8 != (scales is not None):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: an 8-bit output comes with scales, and only that")
+    if not (0.0 < eps < float("inf")):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: eps must be positive and finite")
+    x, ld_in = _norm_operand(client, input, shape, input.dtype, f"{what}: input")
+    res, ld_res = _norm_operand(client, residual, shape, input.dtype, f"{what}: residual")
+    if residual_out is not None and (tuple(residual_out.shape) != shape or residual_out.dtype != input.dtype):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: residual_out must have input's shape and dtype")
+    _flat(weight, (cols,), (ElemType.F32, input.dtype), f"{what}: weight")
+    _flat(rstd, shape[:-1], (ElemType.F32,), f"{what}: rstd")
+    rows, _, ld_out = _norm_rows(output, f"{what}: output")
+    ld_hidden = _norm_rows(residual_out, f"{what}: residual_out")[2] if residual_out is not None else 0
+    block, ld_scales = 0, 0
+    if f8 and scales.dtype == ElemType.UE8M0:
+        block = 32
+        if cols % 32 or tuple(scales.shape) != shape[:-1] + (cols // 32,):
+            raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: ue8m0 scales of shape {tuple(scales.shape)} for {shape} in blocks of 32")
+        ld_scales = _norm_rows(scales, f"{what}: scales")[2]
+    elif f8:
+        _flat(scales, shape[:-1], (ElemType.F32,), f"{what}: scales")
+    desc = N.RmsNormDesc(rows=rows, cols=cols, ld_in=ld_in, ld_residual=ld_res, ld_hidden=ld_hidden, ld_out=ld_out, ld_scales=ld_scales, eps=eps,
+                         dtype=int(input.dtype), dtype_weight=int(weight.dtype) if weight is not None else N.DTYPE_F32, dtype_out=int(output.dtype),
+                         scale_block=block)
+    client._s.check(client.lib.mi355_rms_norm(
+        client.ctx, client.on(x, res, weight, residual_out, output, scales, rstd), C.byref(desc), C.c_void_p(x.device_ptr()), _ptr(res), _ptr(weight),
+        _ptr(residual_out), C.c_void_p(output.device_ptr()), _ptr(scales), _ptr(rstd)))
+
+
+def rms_norm_backward(client: ComputeClient, grad_output: TensorHandle, hidden: TensorHandle, weight: Optional[TensorHandle], rstd: TensorHandle,
+                      grad_input: TensorHandle, *, grad_weight: Optional[TensorHandle] = None, grad_hidden: Optional[TensorHandle] = None) -> None:
+    """The gradient of rms_norm (mi355_rms_norm_grad), x^ = hidden * rstd:
+
+        grad_input = rstd * (w g - x^ mean(w g x^)) + grad_hidden       grad_weight = sum over rows of g x^
+
+    `hidden`: what rms_norm left in residual_out (its input where nothing was added); `rstd` as it left it.  grad_hidden: the gradient that
+    reaches hidden by the residual stream.  grad_input is the gradient of rms_norm's input and of its residual; it may be grad_output,
+    hidden or grad_hidden itself.  grad_weight: [cols], f32 or grad_output's dtype."""
+    what = "rms_norm_backward"
+    dt = grad_output.dtype
+    if dt not in (ElemType.F32, ElemType.BF16, ElemType.F16):
+        raise ServerError(N.E_UNSUPPORTED, f"{what}: operands must be f32, bf16 or f16")
+    if grad_output.rank() == 0:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: rank-0 tensor")
+    shape, cols = tuple(grad_output.shape), grad_output.shape[-1]
+    g, ld_out = _norm_operand(client, grad_output, shape, dt, f"{what}: grad_output")
+    h, ld_hidden = _norm_operand(client, hidden, shape, dt, f"{what}: hidden")
+    s, ld_stream = _norm_operand(client, grad_hidden, shape, dt, f"{what}: grad_hidden")
+    if tuple(grad_input.shape) != shape or grad_input.dtype != dt:
+        raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_input must have grad_output's shape and dtype")
+    _flat(weight, (cols,), (ElemType.F32, dt), f"{what}: weight")
+    _flat(rstd, shape[:-1], (ElemType.F32,), f"{what}: rstd")
+    _flat(grad_weight, (cols,), (ElemType.F32, dt), f"{what}: grad_weight")
+    rows, _, ld_in = _norm_rows(grad_input, f"{what}: grad_input")
+    desc = N.RmsNormGradDesc(rows=rows, cols=cols, ld_out=ld_out, ld_hidden=ld_hidden, ld_in=ld_in, ld_stream=ld_stream, dtype=int(dt),
+                             dtype_weight=int(weight.dtype) if weight is not None else N.DTYPE_F32,
+                             dtype_grad_weight=int(grad_weight.dtype) if grad_weight is not None else N.DTYPE_F32)
+    ws, need = None, C.c_uint64()
+    if grad_weight is not None:
+        client._s.check(client.lib.mi355_rms_norm_grad_workspace_bytes(C.byref(desc), C.byref(need)))
+        if need.value:
+            ws = client.empty(need.value)
+    client._s.check(client.lib.mi355_rms_norm_grad(
+        client.ctx, client.on(g, h, weight, rstd, s, grad_input, grad_weight, ws), C.byref(desc), C.c_void_p(g.device_ptr()), C.c_void_p(h.device_ptr()),
+        _ptr(weight), C.c_void_p(rstd.device_ptr()), _ptr(s), C.c_void_p(grad_input.device_ptr()), _ptr(grad_weight), _ptr(ws), need.value))
+
+
+class TensorList:
+    """Tensors that are used together (a model's gradients): f32, bf16 or f16, each contiguous or with padded rows.  Keep it as long as the
+    tensors' memory: global_norm and clip_by_global_norm then take it without going through the tensors again."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.memories = list({id(t.handle.memory): t.handle for t in self.tensors}.values())    # one handle per allocation, for stream order
+        self.spans = (N.TensorSpan * max(len(self.tensors), 1))()
+        for i, t in enumerate(self.tensors):
+            if t.dtype not in (ElemType.F32, ElemType.BF16, ElemType.F16):
+                raise ServerError(N.E_UNSUPPORTED, f"TensorList: tensor {i} must be f32, bf16 or f16")
+            if t.is_contiguous():
+                self.spans[i] = (t.device_ptr(), 1, t.num_elems(), t.num_elems(), int(t.dtype), 0)
+            else:
+                rows, cols, stride = _norm_rows(t, f"TensorList: tensor {i}")
+                self.spans[i] = (t.device_ptr(), rows, cols, stride, int(t.dtype), 0)
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+
+def _tensor_list(tensors) -> TensorList:
+    return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+
+
+def _norm_workspace(client: ComputeClient) -> Handle:
+    need = C.c_uint64()
+    client._s.check(client.lib.mi355_global_norm_workspace_bytes(C.byref(need)))
+    return client.empty(need.value)                 # the pool's: stream-ordered, and a captured graph keeps its own
+
+
+def global_norm(client: ComputeClient, tensors, output: TensorHandle) -> None:
+    """output[0] (f32) = sqrt(sum of x^2 over all elements of all tensors), summed in f64 in a fixed order (mi355_global_norm).  `tensors`: a
+    TensorList or any sequence of tensors."""
+    tensors = _tensor_list(tensors)
+    _flat(output, (1,), (ElemType.F32,), "global_norm: output")
+    ws = _norm_workspace(client)
+    client._s.check(client.lib.mi355_global_norm(client.ctx, client.on(*tensors.memories, output, ws), tensors.spans, len(tensors),
+                                                 C.c_void_p(output.device_ptr()), C.c_void_p(ws.device_ptr()), ws.size))
+
+
+def clip_by_global_norm(client: ComputeClient, tensors, max_norm: float, *, outputs=None, total_norm: Optional[TensorHandle] = None) -> None:
+    """Every tensor times min(1, max_norm / norm), norm as global_norm gives it, in place or into `outputs` (shapes and dtypes alike)
+    (mi355_clip_by_global_norm).  total_norm (f32) receives the norm.  A NaN or infinite norm makes every output NaN.  `tensors` and
+    `outputs`: TensorLists or any sequences of tensors; no two of them may share memory, in place aside."""
+    tensors = _tensor_list(tensors)
+    outputs = tensors if outputs is None else _tensor_list(outputs)
+    if not max_norm > 0.0:
+        raise ServerError(N.E_INVALID_ARGUMENT, "clip_by_global_norm: max_norm must be positive")
+    _flat(total_norm, (1,), (ElemType.F32,), "clip_by_global_norm: total_norm")
+    if len(outputs) != len(tensors):
+        raise ServerError(N.E_INVALID_ARGUMENT, f"clip_by_global_norm: {len(outputs)} outputs for {len(tensors)} tensors")
+    ins, outs = tensors.spans, outputs.spans
+    if outs is not ins:
+        ins, outs = _span_pairs(tensors, outputs)
+    ws = _norm_workspace(client)
+    handles = tensors.memories if outputs is tensors else tensors.memories + outputs.memories
+    client._s.check(client.lib.mi355_clip_by_global_norm(client.ctx, client.on(*handles, total_norm, ws), ins, outs, len(tensors), max_norm,
+                                                         _ptr(total_norm), C.c_void_p(ws.device_ptr()), ws.size))
+
+
+def _span_pairs(tensors: TensorList, outputs: TensorList):
+    """The spans of both sides, walked the same way: where one of a pair is contiguous and the other has padded rows, both go by rows."""
+    alike = True
+    for a, b in zip(tensors.tensors, outputs.tensors):
+        if tuple(a.shape) != tuple(b.shape) or a.dtype != b.dtype:
+            raise ServerError(N.E_INVALID_ARGUMENT, f"clip_by_global_norm: output {tuple(b.shape)} {b.dtype.name} for {tuple(a.shape)} {a.dtype.name}")
+        alike = alike and a.is_contiguous() == b.is_contiguous()
+    if alike:
+        return tensors.spans, outputs.spans
+    sides = []
+    for side in (tensors, outputs):
+        spans = (N.TensorSpan * max(len(side), 1))()
+        for i, t in enumerate(side.tensors):
+            rows, cols, stride = _norm_rows(t, f"clip_by_global_norm: tensor {i}") if t.rank() else (1, 1, 1)
+            spans[i] = (t.device_ptr(), rows, cols, stride, int(t.dtype), 0)
+        sides.append(spans)
+    return sides

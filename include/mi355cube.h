@@ -471,6 +471,50 @@ int32_t mi355_gemm_scaled(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_
                           const void *a_scales, const void *b, const void *b_scales, void *c);
 int32_t mi355_gemm_scaled_select(mi355_ctx *ctx, const mi355_gemm_scaled_desc *desc, int32_t *out_algo);
 
+/* Matrix product with its epilogue: C = act(rs[m] * cs[n] * (A * B) + bias[n]) + residual, formed in f32 and rounded once to dtype_c -- a linear
+ * layer in one pass over its output.  `desc` as mi355_gemm; every part of the epilogue is optional (NULL / MI355_ACT_NONE).
+ *   bias          n values, dtype_bias F32 or dtype_c; batch entry b reads bias + b * stride_bias (0: one bias for all)
+ *   residual      C's shape and type, rows ld_residual apart; may be C itself (same leading dimension and batch stride)
+ *   pre           if not NULL, receives the activation's argument (what mi355_gemm_fused_grad wants), C's shape and type
+ *   row_scale, col_scale   f32; element i of batch entry b is at i * inc + b * stride (inc 0: one scale for all).  8-bit operands that
+ *                 were quantised by row (mi355_rms_norm) and by column, or by tensor, are multiplied back here.
+ * Outputs must not overlap operands or each other (residual == C above excepted); an overlap that can be told from the descriptors is refused.
+ * NaN and infinities follow the formula; an activation of -inf is its limit (0 for relu, gelu and silu).
+ * The exponentials are v_exp_f32 (relative error below 2^-22 for |z| < 1), erf is Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7).
+ * Kernels that cannot run their epilogue in place write the f32 product to library-owned per-stream scratch first (batch x M x N x 4 bytes):
+ * inside a capture window such a call needs one earlier call of the same size on that stream. */
+enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_GELU = 2 /* z * Phi(z) */, MI355_ACT_GELU_TANH = 3 /* its tanh form */, MI355_ACT_SILU = 4 };
+typedef struct {
+    const void *bias, *residual;
+    void *pre;
+    const float *row_scale, *col_scale;
+    int64_t stride_bias;
+    int64_t ld_residual, stride_residual;
+    int64_t ld_pre, stride_pre;
+    int64_t inc_row_scale, stride_row_scale, inc_col_scale, stride_col_scale;
+    int32_t activation, dtype_bias;
+} mi355_gemm_epilogue;
+int32_t mi355_gemm_fused(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const mi355_gemm_epilogue *epilogue,
+                         const void *a, const void *b, void *c);
+/* 1 in *out_fused: mi355_gemm_fused runs this descriptor's epilogue inside the product's kernel (or its split-K fold); 0: as a pass over the f32
+ * product in scratch.  Host-side only, operands taken as 16-byte aligned. */
+int32_t mi355_gemm_fused_plan(const mi355_gemm_desc *desc, int32_t *out_fused);
+
+/* The epilogue's gradient: grad_pre = grad_out * act'(pre), grad_bias[n] = sum over the rows of that product before its rounding.  pre and
+ * grad_pre have grad_out's type (F32, BF16, F16); pre may be NULL for MI355_ACT_NONE, grad_bias may be NULL, and so may grad_pre where only
+ * the sums are wanted.  grad_pre may be grad_out or pre itself.  batch_bias 0: one bias for all batch entries (the sums run over the batch
+ * too); 1: grad_bias is [batch][n].  Sums are f32 in a fixed order: rows of a slab in sequence, slabs in sequence.
+ * Workspace: mi355_gemm_fused_grad_workspace_bytes, caller-owned; unused (and may be NULL) when grad_bias is. */
+typedef struct {
+    int64_t m, n, batch;
+    int64_t ld_out, ld_pre, ld_grad;               /* grad_out, pre, grad_pre */
+    int64_t stride_out, stride_pre, stride_grad;
+    int32_t dtype, activation, dtype_bias, batch_bias;
+} mi355_gemm_fused_grad_desc;
+int32_t mi355_gemm_fused_grad_workspace_bytes(const mi355_gemm_fused_grad_desc *desc, uint64_t *out_bytes);
+int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_fused_grad_desc *desc, const void *grad_out, const void *pre,
+                              void *grad_pre, void *grad_bias, void *workspace, uint64_t workspace_bytes);
+
 /* =================================== Reductions ========================================== */
 
 /* Bytes of device workspace the array-wide reductions need for `n` elements (one partial
@@ -597,6 +641,58 @@ int32_t mi355_plane_op_f32(mi355_ctx *ctx, mi355_stream stream, const float *in,
  * (1 on the diagonal in `dtype`, 0 elsewhere) into rows `ld` elements apart (ld >= dim; the padding of a pitched
  * allocation is left alone).  dtype: any float, integer or fp8 type of this header. */
 int32_t mi355_fill_identity(mi355_ctx *ctx, mi355_stream stream, void *out, int32_t dtype, uint64_t dim, uint64_t ld);
+
+/* =================================== Norms over rows and over tensors ==================== */
+
+/* Root-mean-square norm of rows, the residual's addition before it and 8-bit rounding after it in one pass:
+ *     h = in + residual        rstd = 1 / sqrt(mean(h^2) + eps)        y = h * rstd * weight
+ * in, residual, hidden (receives h, rounded once; may be in or residual itself) have dtype F32, BF16 or F16; weight [cols] has dtype_weight
+ * F32 or dtype and may be NULL (ones).  The norm is taken of h before its rounding.  rstd: [rows] f32, may be NULL.  residual / hidden may be
+ * NULL.  eps > 0.  Rows whose squares pass the f32 range are summed again 2^-80 smaller.
+ * dtype_out F32 or dtype: out = y.  dtype_out F8E4M3 / F8E5M2: out = y / scale to nearest even, with `scales` by scale_block:
+ *   0    one f32 per row, max|y| / MAX (MAX = 448 / 57344; 1 for a row of zeros, at least FLT_MIN): mi355_gemm_fused takes it as row_scale
+ *   32   one ue8m0 per 32 columns, the least power of two with max|y| / scale <= MAX (1 for zeros): nothing saturates; mi355_gemm_scaled takes
+ *        it as a_scales.  cols must be a multiple of 32.
+ * A row (block) that holds a NaN or an infinity gets a NaN scale. */
+typedef struct {
+    int64_t rows, cols;
+    int64_t ld_in, ld_residual, ld_hidden, ld_out, ld_scales;   /* elements between rows; ld_scales for scale_block 32 */
+    float eps;
+    int32_t dtype, dtype_weight, dtype_out, scale_block, reserved;
+} mi355_rms_norm_desc;
+int32_t mi355_rms_norm(mi355_ctx *ctx, mi355_stream stream, const mi355_rms_norm_desc *desc, const void *in, const void *residual,
+                       const void *weight, void *hidden, void *out, void *scales, float *rstd);
+/* Its gradient, x^ = hidden * rstd:
+ *     grad_in = rstd * (w * g - x^ * mean(w * g * x^)) + grad_hidden        grad_weight = sum over rows of g * x^
+ * grad_out (g), hidden, grad_in and grad_hidden (the gradient that reaches h by the residual stream; may be NULL, or grad_in itself) have
+ * `dtype`; grad_weight (may be NULL) F32 or dtype.  grad_in may also be grad_out or hidden itself.  grad_in is the gradient of `in` and of `residual` alike.
+ * Sums are f32 in a fixed order.  Workspace: mi355_rms_norm_grad_workspace_bytes, caller-owned; unused (may be NULL) when grad_weight is. */
+typedef struct {
+    int64_t rows, cols;
+    int64_t ld_out, ld_hidden, ld_in, ld_stream;                /* grad_out, hidden, grad_in, grad_hidden */
+    int32_t dtype, dtype_weight, dtype_grad_weight, reserved;
+} mi355_rms_norm_grad_desc;
+int32_t mi355_rms_norm_grad_workspace_bytes(const mi355_rms_norm_grad_desc *desc, uint64_t *out_bytes);
+int32_t mi355_rms_norm_grad(mi355_ctx *ctx, mi355_stream stream, const mi355_rms_norm_grad_desc *desc, const void *grad_out, const void *hidden,
+                            const void *weight, const float *rstd, const void *grad_hidden, void *grad_in, void *grad_weight, void *workspace,
+                            uint64_t workspace_bytes);
+
+/* One tensor of a list: `rows` rows of `cols` elements, row_stride elements apart (a contiguous tensor is one row). */
+typedef struct {
+    void *data;
+    uint64_t rows, cols, row_stride;
+    int32_t dtype, reserved;   /* F32, BF16, F16 */
+} mi355_tensor_span;
+/* out_norm[0] = sqrt(sum over all elements of all tensors of x^2), f32.  Squares and sums are f64 (no f32 element over- or underflows), in a
+ * fixed order.  No tensor, or only empty ones: 0.  Workspace (mi355_global_norm_workspace_bytes, a constant; one call at a time). */
+int32_t mi355_global_norm_workspace_bytes(uint64_t *out_bytes);
+int32_t mi355_global_norm(mi355_ctx *ctx, mi355_stream stream, const mi355_tensor_span *tensors, uint32_t count, float *out_norm, void *workspace,
+                          uint64_t workspace_bytes);
+/* out = in * min(1, max_norm / norm) for every tensor of the list, norm as above; out[i] has in[i]'s rows, cols and dtype and may be in[i] itself.
+ * A norm that is NaN or infinite makes every output NaN: no factor brings it to max_norm.  max_norm > 0 (infinity: only the norm is taken
+ * and the tensors copied).  out_norm may be NULL.  Outputs must not overlap each other or another tensor of the list: refused. */
+int32_t mi355_clip_by_global_norm(mi355_ctx *ctx, mi355_stream stream, const mi355_tensor_span *in, const mi355_tensor_span *out, uint32_t count,
+                                  float max_norm, float *out_norm, void *workspace, uint64_t workspace_bytes);
 
 /* =================================== Strided copies (into_contiguous) =================================== */
 

@@ -70,6 +70,11 @@ pub const MI355_REDUCE_MIN: i32 = 3;
 pub const MI355_REDUCE_PROD: i32 = 4;
 pub const MI355_REDUCE_ARGMAX: i32 = 5;
 pub const MI355_REDUCE_ARGMIN: i32 = 6;
+pub const MI355_ACT_NONE: i32 = 0;
+pub const MI355_ACT_RELU: i32 = 1;
+pub const MI355_ACT_GELU: i32 = 2;
+pub const MI355_ACT_GELU_TANH: i32 = 3;
+pub const MI355_ACT_SILU: i32 = 4;
 pub const MI355_UNIQUE_ID_BYTES: usize = 128;
 
 #[repr(C)]
@@ -195,6 +200,89 @@ pub struct mi355_gemm_desc {
     pub reserved: i32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mi355_gemm_epilogue {
+    pub bias: *const c_void,
+    pub residual: *const c_void,
+    pub pre: *mut c_void,
+    pub row_scale: *const f32,
+    pub col_scale: *const f32,
+    pub stride_bias: i64,
+    pub ld_residual: i64,
+    pub stride_residual: i64,
+    pub ld_pre: i64,
+    pub stride_pre: i64,
+    pub inc_row_scale: i64,
+    pub stride_row_scale: i64,
+    pub inc_col_scale: i64,
+    pub stride_col_scale: i64,
+    pub activation: i32,
+    pub dtype_bias: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mi355_gemm_fused_grad_desc {
+    pub m: i64,
+    pub n: i64,
+    pub batch: i64,
+    pub ld_out: i64,
+    pub ld_pre: i64,
+    pub ld_grad: i64,
+    pub stride_out: i64,
+    pub stride_pre: i64,
+    pub stride_grad: i64,
+    pub dtype: i32,
+    pub activation: i32,
+    pub dtype_bias: i32,
+    pub batch_bias: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mi355_rms_norm_desc {
+    pub rows: i64,
+    pub cols: i64,
+    pub ld_in: i64,
+    pub ld_residual: i64,
+    pub ld_hidden: i64,
+    pub ld_out: i64,
+    pub ld_scales: i64,
+    pub eps: f32,
+    pub dtype: i32,
+    pub dtype_weight: i32,
+    pub dtype_out: i32,
+    pub scale_block: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mi355_rms_norm_grad_desc {
+    pub rows: i64,
+    pub cols: i64,
+    pub ld_out: i64,
+    pub ld_hidden: i64,
+    pub ld_in: i64,
+    pub ld_stream: i64,
+    pub dtype: i32,
+    pub dtype_weight: i32,
+    pub dtype_grad_weight: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mi355_tensor_span {
+    pub data: *mut c_void,
+    pub rows: u64,
+    pub cols: u64,
+    pub row_stride: u64,
+    pub dtype: i32,
+    pub reserved: i32,
+}
+
 /// mi355_tensor_layout: TensorBinding's shape / strides (elements, outermost axis first).
 #[repr(C)]
 #[derive(Clone, Copy, Default)]
@@ -254,6 +342,26 @@ unsafe extern "C" {
     // cmma::execute(a, b, c, d): D = A * B + C (frontend/cmma.rs:1066-1110)
     pub fn mi355_gemm_add(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_gemm_desc, a: *const c_void, b: *const c_void,
                           c: *const c_void, d: *mut c_void) -> i32;
+    // a linear layer's epilogue, norms over rows and over tensor lists, and their gradients
+    pub fn mi355_gemm_fused(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_gemm_desc, epilogue: *const mi355_gemm_epilogue,
+                            a: *const c_void, b: *const c_void, c: *mut c_void) -> i32;
+    pub fn mi355_gemm_fused_plan(desc: *const mi355_gemm_desc, out_fused: *mut i32) -> i32;
+    pub fn mi355_gemm_fused_grad_workspace_bytes(desc: *const mi355_gemm_fused_grad_desc, out_bytes: *mut u64) -> i32;
+    pub fn mi355_gemm_fused_grad(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_gemm_fused_grad_desc, grad_out: *const c_void,
+                                 pre: *const c_void, grad_pre: *mut c_void, grad_bias: *mut c_void, workspace: *mut c_void,
+                                 workspace_bytes: u64) -> i32;
+    pub fn mi355_rms_norm(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_rms_norm_desc, input: *const c_void,
+                          residual: *const c_void, weight: *const c_void, hidden: *mut c_void, out: *mut c_void, scales: *mut c_void,
+                          rstd: *mut f32) -> i32;
+    pub fn mi355_rms_norm_grad_workspace_bytes(desc: *const mi355_rms_norm_grad_desc, out_bytes: *mut u64) -> i32;
+    pub fn mi355_rms_norm_grad(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_rms_norm_grad_desc, grad_out: *const c_void,
+                               hidden: *const c_void, weight: *const c_void, rstd: *const f32, grad_hidden: *const c_void,
+                               grad_in: *mut c_void, grad_weight: *mut c_void, workspace: *mut c_void, workspace_bytes: u64) -> i32;
+    pub fn mi355_global_norm_workspace_bytes(out_bytes: *mut u64) -> i32;
+    pub fn mi355_global_norm(ctx: *mut mi355_ctx, stream: mi355_stream, tensors: *const mi355_tensor_span, count: u32, out_norm: *mut f32,
+                             workspace: *mut c_void, workspace_bytes: u64) -> i32;
+    pub fn mi355_clip_by_global_norm(ctx: *mut mi355_ctx, stream: mi355_stream, input: *const mi355_tensor_span, out: *const mi355_tensor_span,
+                                     count: u32, max_norm: f32, out_norm: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> i32;
     pub fn mi355_reduce_workspace_bytes(ctx: *mut mi355_ctx, n: u64, out_bytes: *mut u64) -> i32;
     pub fn mi355_reduce_sum_f32(ctx: *mut mi355_ctx, stream: mi355_stream, input: *const f32, n: u64, out: *mut f32,
                                 workspace: *mut c_void, workspace_bytes: u64) -> i32;

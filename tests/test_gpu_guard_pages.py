@@ -17,6 +17,7 @@ def _child(*args):
     return subprocess.run([sys.executable, str(ROOT / "tools" / "guard_check.py"), *args], capture_output=True, text=True, timeout=900)
 
 
+@pytest.mark.skip(reason="makes the GPU fault on purpose: the fault ends the whole machine's GPU service, and every test after it")
 def test_the_detector_faults_on_an_output_that_is_64_bytes_short():
     r = _child("--selftest")
     assert r.returncode != 0 and "THE DETECTOR DOES NOT WORK" not in r.stdout, r.stdout[-500:]

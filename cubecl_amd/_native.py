@@ -271,7 +271,6 @@ PROTOTYPES = {
     "mi355_gemm": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), _P, _P, _P]),
     "mi355_gemm_add": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), _P, _P, _P, _P]),
     "mi355_gemm_fused": (C.c_int32, [_P, _P, C.POINTER(GemmDesc), C.POINTER(GemmEpilogue), _P, _P, _P]),
-    "mi355_gemm_fused_plan": (C.c_int32, [C.POINTER(GemmDesc), _I32P]),
     "mi355_gemm_fused_grad_workspace_bytes": (C.c_int32, [C.POINTER(GemmFusedGradDesc), _U64P]),
     "mi355_gemm_fused_grad": (C.c_int32, [_P, _P, C.POINTER(GemmFusedGradDesc), _P, _P, _P, _P, _P, C.c_uint64]),
     "mi355_rms_norm": (C.c_int32, [_P, _P, C.POINTER(RmsNormDesc), _P, _P, _P, _P, _P, _P, _P]),

@@ -722,7 +722,7 @@ int32_t select_auto(const mi355_gemm_desc &d, const void *a, const void *b, cons
 }
 
 int32_t run_tail_split(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
-                       const tail_plan &p)
+                       const tail_plan &p, const epilogue_args *ep)
 {
     const int64_t esz = (int64_t)dtype_size(d.dtype_ab), csz = (int64_t)dtype_size(d.dtype_c);
     const int64_t ms = p.along_m ? d.m - p.main_extent : d.m, ns = p.along_m ? d.n : d.n - p.main_extent;   // the strip
@@ -744,26 +744,27 @@ int32_t run_tail_split(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, 
         if (!gemm_lp256w4_supports(md, a, b, c)) return MI355_E_UNSUPPORTED;
         // (round 6: whole rounds of full tiles with a 16-bit C -- the persistent 16x16x32 kernel where it takes the main part:
         //  4608 x 4096 x 8192 254.6 -> 240 us, profiles/r06_tail_split_main_on_qm.txt)
-        const int32_t rc = gemm_lp256qm_supports(md, a, b, c) ? launch_gemm_lp256qm(ctx, s, md, a, b, c) : launch_gemm_lp256w4(ctx, s, md, a, b, c);
+        const int32_t rc = !ep && gemm_lp256qm_supports(md, a, b, c) ? launch_gemm_lp256qm(ctx, s, md, a, b, c)
+                           : ep && gemm_lp256m16_supports(md, a, b, c) ? launch_gemm_lp256m16(ctx, s, md, a, b, c, ep)
+                                                                       : launch_gemm_lp256w4(ctx, s, md, a, b, c, nullptr, ep);
         if (rc != MI355_OK) return rc;
     }
     const int32_t rc = launch_gemm_lp256w4(ctx, s, sd, as, bs, slabs);
     if (rc != MI355_OK) return rc;
-    launch_splitk_fold(s, slabs, (uint32_t)p.splits, ms * ns, 1, ms, ns, cs, d.dtype_c, d.ldc, 0);
+    if (ep) launch_epilogue(s, slabs, (uint32_t)p.splits, ms * ns, p.along_m ? epilogue_at(*ep, p.main_extent, 0) : epilogue_at(*ep, 0, p.main_extent), cs, 1, ms, ns, d.ldc, 0);
+    else launch_splitk_fold(s, slabs, (uint32_t)p.splits, ms * ns, 1, ms, ns, cs, d.dtype_c, d.ldc, 0);
     check_launch(ctx, "mi355_gemm(tail split-K fold)");
     return MI355_OK;
 }
 
 }  // namespace
 
-MI355_API int32_t mi355_gemm(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const void *a,
-                             const void *b, void *c)
+namespace {
+
+// mi355_gemm of a validated descriptor, with the epilogue `ep` where one is given
+int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
-    MI355_REQUIRE_CTX(ctx);
-    int32_t rc = validate(ctx, desc, a, b, c);
-    if (rc != -1) return rc;
-    hipStream_t s = stream_of(ctx, stream);
-    mi355_gemm_desc d = *desc;
+    mi355_gemm_desc d = desc;
     int32_t algo = d.algo == MI355_GEMM_ALGO_AUTO ? select_auto(d, a, b, c) : d.algo;
     if (d.algo == MI355_GEMM_ALGO_AUTO && algo == MI355_GEMM_ALGO_GENERIC) {
         mi355_gemm_desc nd;
@@ -788,30 +789,44 @@ MI355_API int32_t mi355_gemm(mi355_ctx *ctx, mi355_stream stream, const mi355_ge
             }
         }
     }
+    // the persistent kernels carry no epilogue: the same tile, one tile a workgroup
+    if (ep && (algo == MI355_GEMM_ALGO_LP_256P || algo == MI355_GEMM_ALGO_LP_256Q || algo == MI355_GEMM_ALGO_LP_256QM))
+        algo = gemm_lp256m16_supports(d, a, b, c) ? MI355_GEMM_ALGO_LP_256M16 : MI355_GEMM_ALGO_LP_256W4;
     // (MI355_W4_TAIL_SPLIT=1, dev: a FORCED 256x256 launch is split as well -- lets tools/ab_algos.py time the split form against the other tiles)
     static const bool split_forced_too = [] { const char *e = getenv("MI355_W4_TAIL_SPLIT"); return e && atoi(e) == 1; }();
     if ((d.algo == MI355_GEMM_ALGO_AUTO || split_forced_too) && algo == MI355_GEMM_ALGO_LP_256W4) {
         tail_plan tp;
-        if (plan_tail_split(d, tp) && run_tail_split(ctx, s, d, a, b, c, tp) == MI355_OK) return MI355_OK;
+        if (plan_tail_split(d, tp) && run_tail_split(ctx, s, d, a, b, c, tp, ep) == MI355_OK) return MI355_OK;
     }
     switch (algo) {
-    case MI355_GEMM_ALGO_GENERIC: return launch_gemm_generic(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_F32_MFMA: return launch_gemm_f32_mfma(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_LP_128: return launch_gemm_lp128(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_LP_256: return launch_gemm_lp256w4(ctx, s, d, a, b, c);      // retired 8-wave kernel: an alias since ABI 8
-    case MI355_GEMM_ALGO_LP_256W4: return launch_gemm_lp256w4(ctx, s, d, a, b, c);
+    case MI355_GEMM_ALGO_GENERIC: return launch_gemm_generic(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_F32_MFMA: return launch_gemm_f32_mfma(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_LP_128: return launch_gemm_lp128(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_LP_256: return launch_gemm_lp256w4(ctx, s, d, a, b, c, nullptr, ep);      // retired 8-wave kernel: an alias since ABI 8
+    case MI355_GEMM_ALGO_LP_256W4: return launch_gemm_lp256w4(ctx, s, d, a, b, c, nullptr, ep);
     case MI355_GEMM_ALGO_LP_256P: return launch_gemm_lp256p(ctx, s, d, a, b, c);
     case MI355_GEMM_ALGO_LP_256Q: return launch_gemm_lp256q(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_SKINNY: return launch_gemm_skinny(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_STREAM64: return launch_gemm_stream64(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_LP_256X128: return launch_gemm_lp256x128(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_NNROWS: return launch_gemm_nnrows(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_LP_256X192: return launch_gemm_lp256x192(ctx, s, d, a, b, c);
-    case MI355_GEMM_ALGO_LP_192X192: return launch_gemm_lp256x192(ctx, s, d, a, b, c, 192);
-    case MI355_GEMM_ALGO_LP_256M16: return launch_gemm_lp256m16(ctx, s, d, a, b, c);
+    case MI355_GEMM_ALGO_SKINNY: return launch_gemm_skinny(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_STREAM64: return launch_gemm_stream64(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_LP_256X128: return launch_gemm_lp256x128(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_NNROWS: return launch_gemm_nnrows(ctx, s, d, a, b, c, ep);
+    case MI355_GEMM_ALGO_LP_256X192: return launch_gemm_lp256x192(ctx, s, d, a, b, c, 256, ep);
+    case MI355_GEMM_ALGO_LP_192X192: return launch_gemm_lp256x192(ctx, s, d, a, b, c, 192, ep);
+    case MI355_GEMM_ALGO_LP_256M16: return launch_gemm_lp256m16(ctx, s, d, a, b, c, ep);
     case MI355_GEMM_ALGO_LP_256QM: return launch_gemm_lp256qm(ctx, s, d, a, b, c);
     default: return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm: unknown algo %d", algo);
     }
+}
+
+}  // namespace
+
+MI355_API int32_t mi355_gemm(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const void *a,
+                             const void *b, void *c)
+{
+    MI355_REQUIRE_CTX(ctx);
+    const int32_t rc = validate(ctx, desc, a, b, c);
+    if (rc != -1) return rc;
+    return run_gemm(ctx, stream_of(ctx, stream), *desc, a, b, c, nullptr);
 }
 
 // cmma::execute(a, b, c, d) at tensor level: D = A * B + C.  The selected kernel writes the f32 product into
@@ -850,8 +865,7 @@ MI355_API int32_t mi355_gemm_add(mi355_ctx *ctx, mi355_stream stream, const mi35
     return MI355_OK;
 }
 
-// act(rs cs (A B) + bias) + residual: the selected kernel writes the f32 product into library-owned per-stream scratch, gemm_epilogue.hip
-// does the rest in one pass and rounds once.
+// act(rs cs (A B) + bias) + residual: the kernel that mi355_gemm would take runs the epilogue on its accumulators (or in the fold of its K slices).
 MI355_API int32_t mi355_gemm_fused(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const mi355_gemm_epilogue *epilogue, const void *a,
                                    const void *b, void *c)
 {
@@ -859,34 +873,10 @@ MI355_API int32_t mi355_gemm_fused(mi355_ctx *ctx, mi355_stream stream, const mi
     if (!epilogue) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: the epilogue is NULL");
     int32_t rc = validate(ctx, desc, a, b, c);
     if (rc != -1) return rc;
-    const mi355_gemm_desc &d = *desc;
-    const mi355_gemm_epilogue &ep = *epilogue;
-    rc = validate_epilogue(ctx, d, ep, a, b, c);
+    rc = validate_epilogue(ctx, *desc, *epilogue, a, b, c);
     if (rc != MI355_OK) return rc;
-    hipStream_t s = stream_of(ctx, stream);
-    void *prod = nullptr;
-    const size_t bytes = (size_t)d.batch * (size_t)d.m * (size_t)d.n * sizeof(float);
-    if (scratch_get(ctx, s, SCRATCH_PRODUCT, bytes, &prod) != MI355_OK)
-        return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm_fused: no scratch for the %zu-byte f32 product (inside a capture window?)", bytes);
-    mi355_gemm_desc pd = d;
-    pd.dtype_c = MI355_DTYPE_F32;
-    pd.ldc = d.n;
-    pd.stride_c = d.m * d.n;
-    // (named kernels that hold a finished 16-bit tile: the same tile without that)
-    if (d.algo == MI355_GEMM_ALGO_LP_256Q) pd.algo = MI355_GEMM_ALGO_LP_256W4;
-    if (d.algo == MI355_GEMM_ALGO_LP_256QM) pd.algo = MI355_GEMM_ALGO_LP_256M16;
-    rc = mi355_gemm(ctx, stream, &pd, a, b, prod);
-    if (rc != MI355_OK) return rc;
-    launch_epilogue(s, static_cast<const float *>(prod), ep, c, d.batch, d.m, d.n, d.dtype_c, d.ldc, d.stride_c);
-    check_launch(ctx, "mi355_gemm_fused");
-    return MI355_OK;
-}
-
-MI355_API int32_t mi355_gemm_fused_plan(const mi355_gemm_desc *desc, int32_t *out_fused)
-{
-    if (!desc || !out_fused) return MI355_E_INVALID_ARGUMENT;
-    *out_fused = 0;
-    return MI355_OK;
+    const epilogue_args ep = make_epilogue(*epilogue, desc->dtype_c);
+    return run_gemm(ctx, stream_of(ctx, stream), *desc, a, b, c, &ep);
 }
 
 // Introspection (no device needed): how mi355_gemm would cut a descriptor that AUTO resolves to the 256x256 kernel.

@@ -16,6 +16,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 namespace mi355 {
 
+struct epilogue_args;       // mi355_gemm_fused: what a launcher below may be given to do on the accumulators (linear_ops.hpp)
+
 struct gemm_args {
     const void *a;
     const void *b;
@@ -115,34 +117,44 @@ __device__ __forceinline__ uint32_t f32x2_to_lp(float lo, float hi)
 }
 
 // host-side kernel launchers (one per translation unit)
-int32_t launch_gemm_generic(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
-int32_t launch_gemm_f32_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
-int32_t launch_gemm_lp128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
-int32_t launch_gemm_lp256x128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
+int32_t launch_gemm_generic(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
+int32_t launch_gemm_f32_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
+int32_t launch_gemm_lp128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
+int32_t launch_gemm_lp256x128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
 int64_t lp128_split_count(const mi355_gemm_desc &d, int64_t cus);   // K slices of the 128x128 kernel's launcher (gemm_lp128.hip), 1 = none
 bool gemm_lp256x128_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 int32_t launch_gemm_lp256w4(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
-                            const void *c_in = nullptr);
+                            const void *c_in = nullptr, const epilogue_args *ep = nullptr);
 int32_t launch_gemm_lp256p(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
 bool gemm_lp256p_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 int32_t launch_gemm_lp256q(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
 bool gemm_lp256q_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 bool gemm_lp256w4_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
-int32_t launch_gemm_lp256x192(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, int tile_rows = 256);   // gemm_lp256w4.hip, NJ = 3 (tile_rows 192: NI = 3 too)
+int32_t launch_gemm_lp256x192(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, int tile_rows = 256,
+                              const epilogue_args *ep = nullptr);   // gemm_lp256w4.hip, NJ = 3 (tile_rows 192: NI = 3 too)
 bool gemm_lp256x192_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
-int32_t launch_gemm_lp256m16(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);   // gemm_lp256m16.hip
+int32_t launch_gemm_lp256m16(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);   // gemm_lp256m16.hip
 bool gemm_lp256m16_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 int32_t launch_gemm_lp256qm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);    // gemm_lp256qm.hip
 bool gemm_lp256qm_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
-int32_t launch_gemm_skinny(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
+int32_t launch_gemm_skinny(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
 bool gemm_skinny_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
-int32_t launch_gemm_nnrows(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
+int32_t launch_gemm_nnrows(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
 bool gemm_nnrows_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 bool gemm_nnrows_ready(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d);   // its scratch exists or may be created now
-int32_t launch_gemm_stream64(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
+int32_t launch_gemm_stream64(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
 bool gemm_stream64_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 // ... its f32 form (gemm_stream64_f32.hip: v_mfma_f32_16x16x4_f32, both operands through per-wave LDS rings); reached through the two above
-int32_t launch_gemm_stream64_f32(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c);
+int32_t launch_gemm_stream64_f32(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c,
+                            const epilogue_args *ep = nullptr);
 bool gemm_stream64_f32_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 int stream64_f32_blocks(const mi355_gemm_desc &d, int cus);
 // block-scaled (MX) form of the same kernel; sa_t / sb_t are the re-arranged scales (gemm_scaled.hip)

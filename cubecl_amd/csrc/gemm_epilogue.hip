@@ -13,57 +13,60 @@ using namespace mi355;
 
 namespace {
 
-// one call for the activation the launch was made for: the switch is uniform, the eight elements go through straight-line code
-__device__ __forceinline__ void act8(int32_t act, float (&z)[8])
-{
-#define ACT(A) case A: { _Pragma("unroll") for (int e = 0; e < 8; ++e) z[e] = act_of<A>(z[e]); } break
-    switch (act) { ACT(MI355_ACT_RELU); ACT(MI355_ACT_GELU); ACT(MI355_ACT_GELU_TANH); ACT(MI355_ACT_SILU); default: break; }
-#undef ACT
-}
-
-// grid.x: columns in 2048s, grid.y: rows, grid.z: batch
+// One run of eight columns a thread, runs counted along the rows (grid.x), batch entries in grid.y; slabs in fours, so that four loads fly.
+template <class INDEX>
 __global__ void __launch_bounds__(256)
-epilogue_kernel(const float *__restrict__ prod, mi355_gemm_epilogue ep, void *c, int64_t m, int64_t n, int64_t batch, int64_t ldc,
-                int64_t stride_c, int32_t dtype_c)
+epilogue_kernel(const float *__restrict__ prod, uint32_t slabs, int64_t slab_stride, epilogue_args ep, void *c, INDEX runs, INDEX per_row, int64_t m, int64_t n,
+                int64_t ldc, int64_t stride_c)
 {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (i >= n) return;
-    const int valid = (int)min((int64_t)8, n - i);
-    for (int64_t b = blockIdx.z; b < batch; b += gridDim.z) {
-        float bias[8], cs[8];
-        if (ep.bias) load8_any(ep.bias, ep.dtype_bias, b * ep.stride_bias + i, valid, bias);
-        if (ep.col_scale) {
+    const int64_t b = blockIdx.y;
+    for (INDEX id = (INDEX)blockIdx.x * 256 + threadIdx.x; id < runs; id += (INDEX)gridDim.x * 256) {
+        const INDEX q = id / per_row;
+        const int64_t row = (int64_t)q, i = (int64_t)(id - q * per_row) * 8;
+        const int valid = (int)min((int64_t)8, n - i);
+        const float *p = prod + (b * m + row) * n;
+        float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        uint32_t s = 0;
+        for (; s + 4 <= slabs; s += 4) {
+            vec8<MI355_DTYPE_F32> t[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) cs[e] = e < valid ? ep.col_scale[b * ep.stride_col_scale + (i + e) * ep.inc_col_scale] : 0.0f;
+            for (int k = 0; k < 4; ++k) t[k] = load8<MI355_DTYPE_F32>(p + (int64_t)(s + k) * slab_stride, i, valid);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] += get(t[k], e);
         }
-        for (int64_t row = blockIdx.y; row < m; row += gridDim.y) {
-            const vec8<MI355_DTYPE_F32> p = load8<MI355_DTYPE_F32>(prod + (b * m + row) * n, i, valid);
-            float z[8];
+        for (; s < slabs; ++s) {
+            const vec8<MI355_DTYPE_F32> t = load8<MI355_DTYPE_F32>(p + (int64_t)s * slab_stride, i, valid);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = get(p, e);
-            if (ep.row_scale) {
-                const float rs = ep.row_scale[b * ep.stride_row_scale + row * ep.inc_row_scale];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] *= rs;
-            }
-            if (ep.col_scale) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] *= cs[e];
-            }
-            if (ep.bias) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] += bias[e];
-            }
-            if (ep.pre) store8_any(ep.pre, dtype_c, b * ep.stride_pre + row * ep.ld_pre + i, valid, z);
-            act8(ep.activation, z);
-            if (ep.residual) {
-                float r[8];
-                load8_any(ep.residual, dtype_c, b * ep.stride_residual + row * ep.ld_residual + i, valid, r);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] += r[e];
-            }
-            store8_any(c, dtype_c, b * stride_c + row * ldc + i, valid, z);
+            for (int e = 0; e < 8; ++e) z[e] += get(t, e);
         }
+        float v[8];
+        const float rs = ep.p.row_scale ? ep.p.row_scale[b * ep.p.stride_row_scale + row * ep.p.inc_row_scale] : 1.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] *= rs * (ep.p.col_scale && e < valid ? ep.p.col_scale[b * ep.p.stride_col_scale + (i + e) * ep.p.inc_col_scale] : 1.0f);
+        if (ep.p.bias) {
+            load8_any(ep.p.bias, ep.p.dtype_bias, b * ep.p.stride_bias + i, valid, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] += v[e];
+        }
+        if (ep.p.pre) store8_any(ep.p.pre, ep.dtype_c, b * ep.p.stride_pre + row * ep.p.ld_pre + i, valid, z);
+        if (ep.kind == ACT_SIGMOID) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = act_sigmoid(z[e], ep.a, ep.b);
+        } else if (ep.kind == ACT_ERF) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = act_erf(z[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = act_linear(z[e], ep.floor);
+        }
+        if (ep.p.residual) {
+            load8_any(ep.p.residual, ep.dtype_c, b * ep.p.stride_residual + row * ep.p.ld_residual + i, valid, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] += v[e];
+        }
+        store8_any(c, ep.dtype_c, b * stride_c + row * ldc + i, valid, z);
     }
 }
 
@@ -129,11 +132,13 @@ void launch_grad(hipStream_t s, int32_t activation, const fused_grad_args &a)
 
 namespace mi355 {
 
-void launch_epilogue(hipStream_t s, const float *prod, const mi355_gemm_epilogue &ep, void *c, int64_t batch, int64_t m, int64_t n, int32_t dtype_c,
-                     int64_t ldc, int64_t stride_c)
+void launch_epilogue(hipStream_t s, const float *prod, uint32_t slabs, int64_t slab_stride, const epilogue_args &ep, void *c, int64_t batch, int64_t m,
+                     int64_t n, int64_t ldc, int64_t stride_c)
 {
-    const dim3 grid((uint32_t)((n + 2047) / 2048), (uint32_t)std::min<int64_t>(m, 65535), (uint32_t)std::min<int64_t>(batch, 1024));
-    hipLaunchKernelGGL(epilogue_kernel, grid, dim3(256), 0, s, prod, ep, c, m, n, batch, ldc, stride_c, dtype_c);
+    const int64_t per_row = (n + 7) / 8, runs = m * per_row;
+    const dim3 grid((uint32_t)std::min<int64_t>((runs + 255) / 256, 1 << 20), (uint32_t)batch);
+    if (runs < (1ll << 31)) hipLaunchKernelGGL((epilogue_kernel<uint32_t>), grid, dim3(256), 0, s, prod, slabs, slab_stride, ep, c, (uint32_t)runs, (uint32_t)per_row, m, n, ldc, stride_c);
+    else hipLaunchKernelGGL((epilogue_kernel<uint64_t>), grid, dim3(256), 0, s, prod, slabs, slab_stride, ep, c, (uint64_t)runs, (uint64_t)per_row, m, n, ldc, stride_c);
 }
 
 void launch_fused_grad(hipStream_t s, int32_t dtype, int32_t activation, const fused_grad_args &a)

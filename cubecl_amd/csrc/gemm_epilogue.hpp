@@ -1,0 +1,184 @@
+// gemm_epilogue.hpp -- the epilogue of mi355_gemm_fused on a GEMM kernel's f32 accumulators:
+//     z = rs[m] cs[n] (A B)[m][n] + bias[n]      (pre = z)      c = act(z) + residual
+//
+// A kernel takes it as a wider argument block, with_epilogue<its arguments>; `has_epilogue` then compiles the plain stores out and one of the two
+// forms below in, and the kernels without it are what they were.
+//   finish_one    one output, for kernels that store by element (few rows, few columns, edges of everything)
+//   tile_finish   a wave's block of 32 rows that has been staged through LDS in f32: eight columns a lane, so the bias and the column scales
+//                 stay in registers over all rows, and everything leaves in whole 16-byte pieces.  AHEAD: the residual's pieces of a block are
+//                 in flight while its accumulators are staged (one workgroup a CU: nothing else hides their latency); without it a piece is
+//                 fetched when it is needed (several workgroups a CU, and half the registers)
+#pragma once
+
+#include <type_traits>
+#include <utility>
+
+#include "rowops.hpp"
+
+namespace mi355 {
+
+template <class BASE> struct with_epilogue : BASE { epilogue_args ep; };
+template <class G> constexpr bool has_epilogue = false;
+template <class B> constexpr bool has_epilogue<with_epilogue<B>> = true;
+template <class BASE>
+with_epilogue<BASE> add_epilogue(const BASE &g, const epilogue_args &ep)
+{
+    with_epilogue<BASE> w;
+    static_cast<BASE &>(w) = g;
+    w.ep = ep;
+    return w;
+}
+
+// The epilogue of the kernel's only argument, read from the kernel argument segment from here on: the compiler may not fetch its two dozen
+// scalars above the K loop, where they would be parked in vector lanes.
+template <class ARGS>
+__device__ __forceinline__ const epilogue_args &epilogue_of()
+{
+    typedef const __attribute__((address_space(4))) char *seg_ptr;
+    seg_ptr p = (seg_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winvalid-offsetof"
+    p += __builtin_offsetof(ARGS, ep);
+#pragma clang diagnostic pop
+    asm volatile("" : "+s"(p));
+    return *(const epilogue_args *)(const char *)p;
+}
+
+// -> the value to store at (row, col) of batch entry b; `pre` is written here
+__device__ __forceinline__ float finish_one(const epilogue_args &ep, int64_t b, int64_t row, int64_t col, float v)
+{
+    if (ep.p.row_scale) v *= ep.p.row_scale[b * ep.p.stride_row_scale + row * ep.p.inc_row_scale];
+    if (ep.p.col_scale) v *= ep.p.col_scale[b * ep.p.stride_col_scale + col * ep.p.inc_col_scale];
+    if (ep.p.bias) v += load1_any(ep.p.bias, ep.p.dtype_bias, b * ep.p.stride_bias + col);
+    if (ep.p.pre) store1_any(ep.p.pre, ep.dtype_c, b * ep.p.stride_pre + row * ep.p.ld_pre + col, v);
+    v = ep.kind == ACT_SIGMOID ? act_sigmoid(v, ep.a, ep.b) : ep.kind == ACT_ERF ? act_erf(v) : act_linear(v, ep.floor);
+    if (ep.p.residual) v += load1_any(ep.p.residual, ep.dtype_c, b * ep.p.stride_residual + row * ep.p.ld_residual + col);
+    return v;
+}
+// ... of a kernel that knows the output as (small operand's row, large operand's row)
+__device__ __forceinline__ float finish_small_big(const epilogue_args &ep, int64_t b, int64_t small_, int64_t big, float v)
+{
+    return finish_one(ep, b, ep.swapped ? big : small_, ep.swapped ? small_ : big, v);
+}
+
+// LPR lanes a row (columns / 8), 32 rows a block
+template <int DT_C, int LPR, bool AHEAD>
+struct tile_finish {
+    static constexpr int RPI = 64 / LPR, PIECES = 32 / RPI;      // rows a wave instruction covers, pieces of a lane
+    const epilogue_args &ep;
+    int64_t b, row, col, m, ldc, stride_c;
+    char *c;
+    int valid;
+    float bias[8], cs[8], rs[AHEAD ? PIECES : 1];
+    vec8<DT_C> res[AHEAD ? PIECES : 1];
+
+    // the lane's first row and column of the wave's block; `live` false: a lane beyond the block's columns
+    __device__ __forceinline__ tile_finish(const epilogue_args &e, const gemm_args &g, int64_t batch, int64_t row_, int64_t col_, bool live)
+        : ep(e), b(batch), row(row_), col(col_), m(g.m), ldc(g.ldc), stride_c(g.stride_c), c(static_cast<char *>(g.c)),
+          valid(live ? (int)max((int64_t)0, min((int64_t)8, g.n - col_)) : 0)
+    {
+        if (ep.p.bias) load8_any(ep.p.bias, ep.p.dtype_bias, b * ep.p.stride_bias + col, valid, bias);
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+            if (!ep.p.bias) bias[e8] = 0.0f;
+            cs[e8] = ep.p.col_scale && e8 < valid ? ep.p.col_scale[b * ep.p.stride_col_scale + (col + e8) * ep.p.inc_col_scale] : 1.0f;
+        }
+    }
+    // the residual and the row scales of the block that begins `at` rows further down
+    __device__ __forceinline__ void fetch(int at)
+    {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int it = 0; it < PIECES; ++it) fetch_piece(it, row + at + it * RPI);
+        }
+    }
+    __device__ __forceinline__ void fetch_piece(int slot, int64_t r)
+    {
+        const bool in = r < m && valid > 0;
+        rs[slot] = ep.p.row_scale && in ? ep.p.row_scale[b * ep.p.stride_row_scale + r * ep.p.inc_row_scale] : 1.0f;
+        if (ep.p.residual && in) res[slot] = load8<DT_C>(ep.p.residual, b * ep.p.stride_residual + r * ep.p.ld_residual + col, valid);
+    }
+    template <int KIND>
+    __device__ __forceinline__ void piece(const char *rd, int64_t r, int slot)
+    {
+        if (r >= m || valid <= 0) return;
+        const f32x4 lo = *reinterpret_cast<const f32x4 *>(rd), hi = *reinterpret_cast<const f32x4 *>(rd + 16);
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) * (rs[slot] * cs[e]) + bias[e];
+        if (ep.p.pre) store8<DT_C, true>(ep.p.pre, b * ep.p.stride_pre + r * ep.p.ld_pre + col, valid, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            z[e] = KIND == ACT_SIGMOID ? act_sigmoid(z[e], ep.a, ep.b) : KIND == ACT_ERF ? act_erf(z[e]) : act_linear(z[e], ep.floor);
+            if (ep.p.residual) z[e] += get(res[slot], e);
+        }
+        store8<DT_C, true>(c, b * stride_c + r * ldc + col, valid, z);
+    }
+    template <int KIND>
+    __device__ __forceinline__ void rows(const char *rd, int pitch, int at)
+    {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int it = 0; it < PIECES; ++it) piece<KIND>(rd + it * RPI * pitch, row + at + it * RPI, it);
+        } else {
+#pragma unroll 1
+            for (int it = 0; it < PIECES; ++it) {
+                fetch_piece(0, row + at + it * RPI);
+                piece<KIND>(rd + it * RPI * pitch, row + at + it * RPI, 0);
+            }
+        }
+    }
+    // All NB blocks: stage(block, as a constant) puts a block's accumulators into LDS, rows `pitch` bytes apart; `rd`: the lane's eight columns of
+    // its first row there.  From three blocks up the loop is a loop -- the accumulators are named by a branch over the block's number, kept apart
+    // by the empty statements (merged, the branches would index the accumulators at run time: out of registers) -- so that the code behind the
+    // staging, a few thousand instructions, is there once.
+    template <int NB, class STAGE>
+    __device__ __forceinline__ void run(STAGE stage, const char *rd, int pitch)
+    {
+        if constexpr (NB <= 2) {
+            one<0>(stage, rd, pitch);
+            if constexpr (NB == 2) one<1>(stage, rd, pitch);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < NB; ++i) {
+                fetch(i * 32);
+                stage_one(std::make_integer_sequence<int, NB>{}, i, stage);
+                finish_block(rd, pitch, i);
+            }
+        }
+    }
+    template <int I, class STAGE>
+    __device__ __forceinline__ void one(STAGE &stage, const char *rd, int pitch)
+    {
+        fetch(I * 32);
+        stage(std::integral_constant<int, I>{});
+        finish_block(rd, pitch, I);
+    }
+    __device__ __forceinline__ void finish_block(const char *rd, int pitch, int i)
+    {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // same-wave hand-over: the DS operations of one wave execute in order
+        block(rd, pitch, i * 32);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    template <int I, class STAGE>
+    static __device__ __forceinline__ void stage_apart(STAGE &stage)
+    {
+        asm volatile("; block %0" ::"i"(I) : "memory");
+        stage(std::integral_constant<int, I>{});
+        asm volatile("; block %0 staged" ::"i"(I) : "memory");
+    }
+    template <int... I, class STAGE>
+    static __device__ __forceinline__ void stage_one(std::integer_sequence<int, I...>, int i, STAGE &stage)
+    {
+        ((i == I ? stage_apart<I>(stage) : (void)0), ...);
+    }
+    // the block's rows, staged `pitch` bytes apart; `rd`: the lane's eight columns of its first row
+    __device__ __forceinline__ void block(const char *rd, int pitch, int at)
+    {
+        if (ep.kind == ACT_SIGMOID) rows<ACT_SIGMOID>(rd, pitch, at);
+        else if (ep.kind == ACT_ERF) rows<ACT_ERF>(rd, pitch, at);
+        else rows<ACT_LINEAR>(rd, pitch, at);
+    }
+};
+
+}  // namespace mi355

@@ -16,7 +16,7 @@
 //
 // Operands are SWAPPED in the MFMA call (first = B fragment, second = A fragment) so that each
 // lane ends up with 4 consecutive N-columns of one C row per register quad => 16-byte stores.
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -31,9 +31,9 @@ struct __attribute__((aligned(16))) f32_smem {
     float b[2][BM * LDK];  // NT: [BN][LDK]; NN: [BK][LDN] (smaller, fits)
 };
 
-template <bool TRANS_B>
+template <bool TRANS_B, class ARGS = gemm_args>
 __global__ void __launch_bounds__(256, 2)
-gemm_f32_mfma_kernel(gemm_args g)
+gemm_f32_mfma_kernel(ARGS g)
 {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     f32_smem &sm = *reinterpret_cast<f32_smem *>(smem_raw);
@@ -160,6 +160,23 @@ gemm_f32_mfma_kernel(gemm_args g)
     }
 
     // ---- epilogue: lane holds C[m][n_base + 0..3] in regs 4q..4q+3 --------------------------
+    if constexpr (has_epilogue<ARGS>) {                    // (never a K slice: the fold has the epilogue there)
+        constexpr int RS = 64 * 4 + 16, STAGE = (32 * RS + 1023) & ~1023, LPR = 8;
+        static_assert(4 * STAGE <= (int)sizeof(f32_smem), "the operand tiles make room for the waves' staged blocks");
+        char *stage = reinterpret_cast<char *>(&sm) + wave * STAGE;      // (the K loop ended in a barrier)
+        char *wr = stage + l31 * RS + 4 * h * 4;
+        const char *rd = stage + (lane / LPR) * RS + (lane % LPR) * 32;
+        tile_finish<MI355_DTYPE_F32, LPR, false> fin(epilogue_of<ARGS>(), g, batch, m0 + wm * 64 + lane / LPR, n0 + wn * 64 + (lane % LPR) * 8, true);
+        fin.template run<2>([&](auto ib) __attribute__((always_inline)) {
+            constexpr int I = decltype(ib)::value;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4 *>(wr + (j * 32 + 8 * q) * 4) = (f32x4){acc[I][j][4 * q + 0], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+        }, rd, RS);
+        return;
+    }
     const bool vec_ok = ((g.ldc & 3) == 0) && ((reinterpret_cast<uintptr_t>(C) & 15u) == 0);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -206,7 +223,7 @@ bool gemm_f32_mfma_supports(const mi355_gemm_desc &d, const void *a, const void 
 }
 
 int32_t launch_gemm_f32_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b,
-                             void *c)
+                             void *c, const epilogue_args *ep)
 {
     if (!gemm_f32_mfma_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "f32 MFMA GEMM: shape/layout not supported by this kernel");
@@ -239,13 +256,20 @@ int32_t launch_gemm_f32_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_des
     const dim3 grid(g.tiles_m * g.tiles_n, (uint32_t)d.batch, (uint32_t)splits);
     const size_t lds = sizeof(f32_smem);
     // the dynamic-LDS attribute is per device: remember it per context, not in a process-wide static
-    const void *fn = d.trans_b ? reinterpret_cast<const void *>(gemm_f32_mfma_kernel<true>)
-                               : reinterpret_cast<const void *>(gemm_f32_mfma_kernel<false>);
-    lds_opt_in(ctx, fn, (int)lds);
-    if (d.trans_b) hipLaunchKernelGGL(gemm_f32_mfma_kernel<true>, grid, dim3(256), lds, s, g);
-    else hipLaunchKernelGGL(gemm_f32_mfma_kernel<false>, grid, dim3(256), lds, s, g);
+    auto go = [&](auto kernel, const auto &args) {
+        lds_opt_in(ctx, reinterpret_cast<const void *>(kernel), (int)lds);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, args);
+    };
+    if (ep && splits == 1) {
+        if (d.trans_b) go(gemm_f32_mfma_kernel<true, with_epilogue<gemm_args>>, add_epilogue(g, *ep));
+        else go(gemm_f32_mfma_kernel<false, with_epilogue<gemm_args>>, add_epilogue(g, *ep));
+    } else if (d.trans_b) go(gemm_f32_mfma_kernel<true>, g);
+    else go(gemm_f32_mfma_kernel<false>, g);
     check_launch(ctx, "mi355_gemm(f32 mfma)");
-    if (splits > 1) {
+    if (splits > 1 && ep) {
+        launch_epilogue(s, ws, (uint32_t)splits, d.batch * d.m * d.n, *ep, c, d.batch, d.m, d.n, d.ldc, d.stride_c);
+        check_launch(ctx, "mi355_gemm_fused(f32 split-K fold)");
+    } else if (splits > 1) {
         launch_splitk_fold(s, ws, (uint32_t)splits, d.batch * d.m * d.n, d.batch, d.m, d.n, c, MI355_DTYPE_F32, d.ldc, d.stride_c);
         check_launch(ctx, "mi355_gemm(f32 split-K fold)");
     }

@@ -2,7 +2,9 @@
 // MFMA kernels do not take (ragged K, transposed A, 16-bit row-major B, unaligned strides).
 // Correctness path, not a roofline path: 64x64x16 tile, 4x4 outputs per thread, f32 FMA chain in
 // k order (the order of runtime_tests/cmma.rs:695-722).
-#include "gemm_common.hpp"
+#include <type_traits>
+
+#include "gemm_epilogue.hpp"
 #include "fp8.hpp"
 
 #include <hip/hip_fp16.h>
@@ -22,11 +24,11 @@ __device__ __forceinline__ float load_as_f32(const void *p, int64_t idx)
     return __half2float(__ushort_as_half(raw));
 }
 
-template <int DT_AB, int DT_C>
+template <int DT_AB, int DT_C, class EP = int>
 __global__ void __launch_bounds__(256)
 gemm_generic_kernel(const void *__restrict__ A, const void *__restrict__ B, void *__restrict__ C, int64_t M, int64_t N,
                     int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int64_t sa, int64_t sb, int64_t sc, int trans_a,
-                    int trans_b, uint32_t tiles_n)
+                    int trans_b, uint32_t tiles_n, EP ep)
 {
     constexpr int BM = 64, BN = 64, BK = 16;
     __shared__ float As[BK][BM + 1];
@@ -90,6 +92,7 @@ gemm_generic_kernel(const void *__restrict__ A, const void *__restrict__ B, void
             const int64_t n = n0 + tx * 4 + j;
             if (n >= N) continue;
             const int64_t idx = oc + m * ldc + n;
+            if constexpr (!std::is_same_v<EP, int>) acc[i][j] = finish_one(ep, batch, m, n, acc[i][j]);
             if (DT_C == MI355_DTYPE_F32) static_cast<float *>(C)[idx] = acc[i][j];
             else static_cast<uint16_t *>(C)[idx] = f32_to_lp<DT_C>(acc[i][j]);
         }
@@ -97,12 +100,15 @@ gemm_generic_kernel(const void *__restrict__ A, const void *__restrict__ B, void
 }
 
 template <int DT_AB, int DT_C>
-void launch(hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+void launch(hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     const uint32_t tiles_m = (uint32_t)((d.m + 63) / 64), tiles_n = (uint32_t)((d.n + 63) / 64);
-    hipLaunchKernelGGL((gemm_generic_kernel<DT_AB, DT_C>), dim3(tiles_m * tiles_n, (uint32_t)d.batch), dim3(256), 0, s, a,
-                       b, c, d.m, d.n, d.k, d.lda, d.ldb, d.ldc, d.stride_a, d.stride_b, d.stride_c, d.trans_a,
-                       d.trans_b, tiles_n);
+    auto go = [&](auto kernel, auto e) {
+        hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n, (uint32_t)d.batch), dim3(256), 0, s, a, b, c, d.m, d.n, d.k, d.lda, d.ldb, d.ldc, d.stride_a, d.stride_b,
+                           d.stride_c, d.trans_a, d.trans_b, tiles_n, e);
+    };
+    if (ep) go(gemm_generic_kernel<DT_AB, DT_C, epilogue_args>, *ep);
+    else go(gemm_generic_kernel<DT_AB, DT_C>, 0);
 }
 
 }  // namespace
@@ -110,21 +116,21 @@ void launch(hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *
 namespace mi355 {
 
 int32_t launch_gemm_generic(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b,
-                            void *c)
+                            void *c, const epilogue_args *ep)
 {
     if (d.batch > 65535) return fail(ctx, MI355_E_UNSUPPORTED, "generic GEMM: batch %lld > 65535", (long long)d.batch);
     const int ab = d.dtype_ab, cd = d.dtype_c;
-    if (ab == MI355_DTYPE_F32 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F32, MI355_DTYPE_F32>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_BF16 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_BF16 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F16 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F16 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(s, d, a, b, c);
-    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(s, d, a, b, c);
+    if (ab == MI355_DTYPE_F32 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F32, MI355_DTYPE_F32>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_BF16 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_BF16 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F16 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F16 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E4M3 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(s, d, a, b, c, ep);
+    else if (ab == MI355_DTYPE_F8E5M2 && cd == MI355_DTYPE_F16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(s, d, a, b, c, ep);
     else return fail(ctx, MI355_E_UNSUPPORTED, "generic GEMM: unsupported dtypes ab=%d c=%d", ab, cd);
     check_launch(ctx, "mi355_gemm(generic)");
     return MI355_OK;

@@ -25,7 +25,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -130,11 +130,11 @@ __device__ __forceinline__ uint32_t lds_addr_of(const void *p)
 // (MI355X_MICROARCH.md, "LDS-DMA piece issue cost"); at eight pieces per wave and K-tile that is more than the 512 cycles
 // the K-tile's 16 MFMAs take, so a wave that does both starves its matrix pipe.  The loader waves own `vmcnt`; the
 // multiplying waves see the ring only through the one s_barrier per K-tile.
-template <int DT, int DT_C, int NS = 2, bool SPEC = false, bool BNN = false, int MI = 2, bool ATN = false>
+template <int DT, int DT_C, int NS = 2, bool SPEC = false, bool BNN = false, int MI = 2, bool ATN = false, class ARGS = gemm_args>
 __global__ void __launch_bounds__(SPEC ? 512 : 256,
                                   // waves per SIMD the register budget must allow (fp8 fragments are twice as wide: three, not four)
                                   NS == 1 ? ((DT == MI355_DTYPE_F8E4M3 || DT == MI355_DTYPE_F8E5M2) ? 3 : 4) : NS == 2 ? (SPEC ? 4 : 2) : SPEC ? 2 : 1)
-gemm_lp128_kernel(gemm_args g)
+gemm_lp128_kernel(ARGS g)
 {
     static_assert(!SPEC || NS == 4 || NS == 3 || NS == 2, "loader waves are written for the 2-stage ring and the deep rings");
     static_assert(MI == 1 || MI == 2 || (MI == 4 && NS == 3 && DT != MI355_DTYPE_F8E4M3 && DT != MI355_DTYPE_F8E5M2), "256 x 128 tile: three-stage ring, 16-bit operands");
@@ -546,6 +546,24 @@ gemm_lp128_kernel(gemm_args g)
         if (t == 12345.678f) static_cast<float *>(g.c)[0] = t;
         return;
     }
+    if constexpr (has_epilogue<ARGS>) {                    // (never a K slice: the fold has the epilogue there)
+        constexpr int RS = 64 * 4 + 16, STAGE = (32 * RS + 1023) & ~1023, LPR = 8;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();                                   // every wave is done with the operand tiles: LDS is free
+        char *stage = smem + wave * STAGE;
+        char *wr = stage + l31 * RS + 4 * h * 4;
+        const char *rd = stage + (lane / LPR) * RS + (lane % LPR) * 32;
+        tile_finish<DT_C, LPR, false> fin(epilogue_of<ARGS>(), g, batch, m0 + wm * 32 * MI + lane / LPR, n0 + wn * 64 + (lane % LPR) * 8, true);
+        fin.template run<MI>([&](auto ib) __attribute__((always_inline)) {
+            constexpr int I = decltype(ib)::value;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4 *>(wr + (j * 32 + 8 * q) * 4) = (f32x4){acc[I][j][4 * q + 0], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+        }, rd, RS);
+        return;
+    }
     char *__restrict__ C = static_cast<char *>(g.c);
     constexpr int CSZ = (DT_C == MI355_DTYPE_F32) ? 4 : 2;
     const int64_t cbase = batch * g.stride_c + (int64_t)z * g.split_c_stride;
@@ -659,15 +677,15 @@ gemm_lp128_kernel(gemm_args g)
 #ifndef LP128_SPEC
 #define LP128_SPEC 1   // dev: 0 = the 4-stage ring without loader waves
 #endif
-template <int DT, int DT_C, int NS, bool SPEC = false, bool BNN = false, int MI = 2, bool ATN = false>
-void launch_ns(mi355_ctx *ctx, hipStream_t s, const gemm_args &g, uint32_t batch)
+template <int DT, int DT_C, int NS, bool SPEC = false, bool BNN = false, int MI = 2, bool ATN = false, class ARGS>
+void launch_ns(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     // operand stages, or the four per-wave epilogue scratch areas when those are larger (f32 C with one stage: 36 KiB)
-    constexpr int CSZ_ = DT_C == MI355_DTYPE_F32 ? 4 : 2;
+    constexpr int CSZ_ = DT_C == MI355_DTYPE_F32 || has_epilogue<ARGS> ? 4 : 2;
     constexpr int EPI = 4 * ((32 * (64 * CSZ_ + 16) + 1023) & ~1023);
     constexpr int LDS = NS * geom<MI>::STAGE > EPI ? NS * geom<MI>::STAGE : EPI;
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp128_kernel<DT, DT_C, NS, SPEC, BNN, MI, ATN>), LDS);
-    hipLaunchKernelGGL((gemm_lp128_kernel<DT, DT_C, NS, SPEC, BNN, MI, ATN>), dim3(g.tiles_m * g.tiles_n, batch, g.split_k > 1 ? g.split_k : 1),
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp128_kernel<DT, DT_C, NS, SPEC, BNN, MI, ATN, ARGS>), LDS);
+    hipLaunchKernelGGL((gemm_lp128_kernel<DT, DT_C, NS, SPEC, BNN, MI, ATN, ARGS>), dim3(g.tiles_m * g.tiles_n, batch, g.split_k > 1 ? g.split_k : 1),
                        dim3(SPEC ? 512 : 256), LDS, s, g);
 }
 
@@ -682,8 +700,8 @@ void launch_ns(mi355_ctx *ctx, hipStream_t s, const gemm_args &g, uint32_t batch
 #ifndef LP128_SMALL_M
 #define LP128_SMALL_M 1   // dev: 0 = the 128 x 128 tile for every M
 #endif
-template <int DT, int DT_C, bool BNN = false, bool ATN = false>
-void launch(mi355_ctx *ctx, hipStream_t s, const gemm_args &g, uint32_t batch)
+template <int DT, int DT_C, bool BNN = false, bool ATN = false, class ARGS>
+void launch(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     if constexpr (LP128_SMALL_M && !ATN && (DT == MI355_DTYPE_BF16 || DT == MI355_DTYPE_F16)) {
         if (g.m <= 64) {
@@ -796,7 +814,7 @@ int64_t lp128_split_count(const mi355_gemm_desc &d, int64_t cus)
 }
 
 int32_t launch_gemm_lp128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b,
-                          void *c)
+                          void *c, const epilogue_args *ep)
 {
     if (!gemm_lp128_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "lp128 GEMM: shape/layout not supported by this kernel");
@@ -833,42 +851,47 @@ int32_t launch_gemm_lp128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &
             else if (d.dtype_ab == MI355_DTYPE_F8E4M3) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(ctx, s, gs, batch);
             else launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(ctx, s, gs, batch);
             check_launch(ctx, "mi355_gemm(lp128 split-K)");
-            launch_splitk_fold(s, ws, (uint32_t)splits, slab, d.batch, d.m, d.n, c, d.dtype_c, d.ldc, d.stride_c);
+            if (ep) launch_epilogue(s, ws, (uint32_t)splits, slab, *ep, c, d.batch, d.m, d.n, d.ldc, d.stride_c);
+            else launch_splitk_fold(s, ws, (uint32_t)splits, slab, d.batch, d.m, d.n, c, d.dtype_c, d.ldc, d.stride_c);
             check_launch(ctx, "mi355_gemm(split-K fold)");
             return MI355_OK;
         }
     }
-    if (d.dtype_ab == MI355_DTYPE_F8E4M3) {
-        if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(ctx, s, g, batch);
-        else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(ctx, s, g, batch);
-        else launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(ctx, s, g, batch);
-    } else if (d.dtype_ab == MI355_DTYPE_F8E5M2) {
-        if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(ctx, s, g, batch);
-        else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(ctx, s, g, batch);
-        else launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(ctx, s, g, batch);
-    } else if (d.dtype_ab == MI355_DTYPE_BF16) {
-        if (d.trans_a) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true, true>(ctx, s, g, batch);
-        } else if (d.trans_b) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(ctx, s, g, batch);
+    auto go = [&](const auto &g) {
+        if (d.dtype_ab == MI355_DTYPE_F8E4M3) {
+            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(ctx, s, g, batch);
+            else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            else launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(ctx, s, g, batch);
+        } else if (d.dtype_ab == MI355_DTYPE_F8E5M2) {
+            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(ctx, s, g, batch);
+            else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            else launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(ctx, s, g, batch);
+        } else if (d.dtype_ab == MI355_DTYPE_BF16) {
+            if (d.trans_a) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true, true>(ctx, s, g, batch);
+            } else if (d.trans_b) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            } else {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true>(ctx, s, g, batch);
+            }
         } else {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true>(ctx, s, g, batch);
+            if (d.trans_a) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true, true>(ctx, s, g, batch);
+            } else if (d.trans_b) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(ctx, s, g, batch);
+            } else {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true>(ctx, s, g, batch);
+            }
         }
-    } else {
-        if (d.trans_a) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true, true>(ctx, s, g, batch);
-        } else if (d.trans_b) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(ctx, s, g, batch);
-        } else {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true>(ctx, s, g, batch);
-        }
-    }
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
     check_launch(ctx, "mi355_gemm(lp128)");
     return MI355_OK;
 }
@@ -882,7 +905,7 @@ bool gemm_lp256x128_supports(const mi355_gemm_desc &d, const void *a, const void
     return gemm_lp128_supports(d, a, b, c);
 }
 
-int32_t launch_gemm_lp256x128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_lp256x128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     if (!gemm_lp256x128_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "lp256x128 GEMM: shape/layout not supported by this kernel");
@@ -898,11 +921,15 @@ int32_t launch_gemm_lp256x128(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_de
     g.split_c_stride = 0;
     const uint32_t batch = (uint32_t)d.batch;
 #define TALL(DT_, DC_) { if (d.trans_b) launch_ns<DT_, DC_, 3, !LP128_INSTREAM, false, 4>(ctx, s, g, batch); else launch_ns<DT_, DC_, 3, !LP128_INSTREAM, true, 4>(ctx, s, g, batch); }
-    if (d.dtype_ab == MI355_DTYPE_BF16) {
-        if (d.dtype_c == MI355_DTYPE_F32) TALL(MI355_DTYPE_BF16, MI355_DTYPE_F32) else TALL(MI355_DTYPE_BF16, MI355_DTYPE_BF16)
-    } else {
-        if (d.dtype_c == MI355_DTYPE_F32) TALL(MI355_DTYPE_F16, MI355_DTYPE_F32) else TALL(MI355_DTYPE_F16, MI355_DTYPE_F16)
-    }
+    auto go = [&](const auto &g) {
+        if (d.dtype_ab == MI355_DTYPE_BF16) {
+            if (d.dtype_c == MI355_DTYPE_F32) TALL(MI355_DTYPE_BF16, MI355_DTYPE_F32) else TALL(MI355_DTYPE_BF16, MI355_DTYPE_BF16)
+        } else {
+            if (d.dtype_c == MI355_DTYPE_F32) TALL(MI355_DTYPE_F16, MI355_DTYPE_F32) else TALL(MI355_DTYPE_F16, MI355_DTYPE_F16)
+        }
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
 #undef TALL
     check_launch(ctx, "mi355_gemm(lp256x128)");
     return MI355_OK;

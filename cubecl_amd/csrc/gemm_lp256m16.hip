@@ -30,7 +30,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -74,9 +74,9 @@ __device__ __forceinline__ uint32_t lds_addr_of(const void *p)
 #define WAIT_LGKM0() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 template <int V> using IC = std::integral_constant<int, V>;
 
-template <int DT, int DT_C>
+template <int DT, int DT_C, class ARGS = gemm_args>
 __global__ void __launch_bounds__(256)
-gemm_lp256m16_kernel(gemm_args g)
+gemm_lp256m16_kernel(ARGS g)
 {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     typedef typename m16<DT>::frag frag;
@@ -252,6 +252,22 @@ gemm_lp256m16_kernel(gemm_args g)
     // With srcA = the B fragment, lane (l15, g) holds for block (i, j): C[m = 16 i + l15][n = 16 j + 4 g .. + 3] -- four consecutive
     // columns of ONE row.  Each wave transposes its 128 x 128 block through its own LDS scratch, 32 rows (two block rows) at a time,
     // and writes whole rows: 16 bytes per lane, 256 (16-bit) / 512 (f32) contiguous bytes per row (as gemm_lp256w4.hip).
+    if constexpr (has_epilogue<ARGS>) {
+        constexpr int RS = 128 * 4 + 16, STAGE = (32 * RS + 1023) & ~1023, LPR = 16;
+        __builtin_amdgcn_s_barrier();                      // every wave is done with the ring
+        char *stage = smem + wave * STAGE;
+        char *wr = stage + l15 * RS + 4 * g4 * 4;
+        const char *rd = stage + (lane / LPR) * RS + (lane % LPR) * 32;
+        tile_finish<DT_C, LPR, true> fin(epilogue_of<ARGS>(), g, batch, m0 + wm * 128 + lane / LPR, n0 + wn * 128 + (lane % LPR) * 8, true);
+        fin.template run<4>([&](auto ip) __attribute__((always_inline)) {      // block rows 2 ip, 2 ip + 1 = 32 rows of the wave's block
+            constexpr int IP = decltype(ip)::value;
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<f32x4 *>(wr + ii * 16 * RS + j * 16 * 4) = acc[2 * IP + ii][j];
+        }, rd, RS);
+        return;
+    }
     char *__restrict__ C = static_cast<char *>(g.c);
     constexpr int CSZ = (DT_C == MI355_DTYPE_F32) ? 4 : 2;
     const int64_t cbase = batch * g.stride_c;
@@ -308,11 +324,11 @@ gemm_lp256m16_kernel(gemm_args g)
     }
 }
 
-template <int DT, int DT_C>
-void launch(mi355_ctx *ctx, hipStream_t s, const gemm_args &g, uint32_t batch)
+template <int DT, int DT_C, class ARGS>
+void launch(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp256m16_kernel<DT, DT_C>), LDS_BYTES);
-    hipLaunchKernelGGL((gemm_lp256m16_kernel<DT, DT_C>), dim3(g.tiles_m * g.tiles_n, batch), dim3(256), LDS_BYTES, s, g);
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp256m16_kernel<DT, DT_C, ARGS>), LDS_BYTES);
+    hipLaunchKernelGGL((gemm_lp256m16_kernel<DT, DT_C, ARGS>), dim3(g.tiles_m * g.tiles_n, batch), dim3(256), LDS_BYTES, s, g);
 }
 
 }  // namespace
@@ -326,7 +342,7 @@ bool gemm_lp256m16_supports(const mi355_gemm_desc &d, const void *a, const void 
     return gemm_lp256w4_supports(d, a, b, c);          // same tile, same operand rules
 }
 
-int32_t launch_gemm_lp256m16(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_lp256m16(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     if (!gemm_lp256m16_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "lp256m16 GEMM: shape/layout not supported by this kernel");
@@ -340,11 +356,15 @@ int32_t launch_gemm_lp256m16(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_des
     g.group_m = M16_GROUP_M;
     const uint32_t batch = (uint32_t)d.batch;
     constexpr int BF = MI355_DTYPE_BF16, HF = MI355_DTYPE_F16, CF = MI355_DTYPE_F32;
-    if (d.dtype_ab == BF) {
-        if (d.dtype_c == CF) launch<BF, CF>(ctx, s, g, batch); else launch<BF, BF>(ctx, s, g, batch);
-    } else {
-        if (d.dtype_c == CF) launch<HF, CF>(ctx, s, g, batch); else launch<HF, HF>(ctx, s, g, batch);
-    }
+    auto go = [&](const auto &g) {
+        if (d.dtype_ab == BF) {
+            if (d.dtype_c == CF) launch<BF, CF>(ctx, s, g, batch); else launch<BF, BF>(ctx, s, g, batch);
+        } else {
+            if (d.dtype_c == CF) launch<HF, CF>(ctx, s, g, batch); else launch<HF, HF>(ctx, s, g, batch);
+        }
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
     check_launch(ctx, "mi355_gemm(lp256m16)");
     return MI355_OK;
 }

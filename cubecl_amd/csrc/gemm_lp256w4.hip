@@ -44,7 +44,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -201,9 +201,9 @@ __device__ __forceinline__ void scale_ld32(uint32_t &dst, const void *ubase, uin
 // 256 x 192).  Same ring, same schedule: a B unit is 24 KiB in its 32 KiB slot (6 DMA pieces per wave instead of 8), the reads,
 // MFMAs and pieces of column fragment 3 are simply not emitted.  Plain [N][K] 16-bit operands only.
 // NI: the same for the rows -- 3 = 192 tile rows (each wave 96 rows): with NJ = 3 a 192 x 192 tile, 9 MFMAs per k-step, 144 accumulators.
-template <int DT, int DT_C, bool BNN = false, int DTB = DT, bool MX = false, bool ATN = false, int NJ = 4, int NI = 4>
+template <int DT, int DT_C, bool BNN = false, int DTB = DT, bool MX = false, bool ATN = false, int NJ = 4, int NI = 4, class ARGS = gemm_args>
 __global__ void __launch_bounds__(256)
-gemm_lp256w4_kernel(gemm_args g)
+gemm_lp256w4_kernel(ARGS g)
 {
     static_assert((NJ == 4 && NI == 4) || ((NJ == 3 || NJ == 4) && (NI == 3 || NI == 4) && !MX && !ATN && (DT == MI355_DTYPE_BF16 || DT == MI355_DTYPE_F16)),
                   "narrow tiles: 16-bit operands, A [M][K], B [N][K] or row-major [K][N]");
@@ -647,6 +647,23 @@ gemm_lp256w4_kernel(gemm_args g)
     // rows at a time, and writes whole rows: 16 B per lane, 256 (16-bit) / 512 (f32) contiguous bytes
     // per row, every line written once.  Row pitch +16 B keeps the b128 accesses aligned and the
     // writes at most 2-way bank conflicted.
+    if constexpr (has_epilogue<ARGS>) {
+        constexpr int RS = 128 * 4 + 16, STAGE = (32 * RS + 1023) & ~1023, LPR = 16;
+        __builtin_amdgcn_s_barrier();                      // every wave's tail DMA has landed; LDS is free
+        char *stage = smem + wave * STAGE;
+        char *wr = stage + l31 * RS + 4 * h * 4;
+        const char *rd = stage + (lane / LPR) * RS + (lane % LPR) * 32;
+        tile_finish<DT_C, LPR, true> fin(epilogue_of<ARGS>(), g, batch, m0 + wm * (NI * 32) + lane / LPR, n0 + wn * (NJ * 32) + (lane % LPR) * 8, (lane % LPR) * 8 < NJ * 32);
+        fin.template run<NI>([&](auto ib) __attribute__((always_inline)) {
+            constexpr int I = decltype(ib)::value;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4 *>(wr + (j * 32 + 8 * q) * 4) = (f32x4){acc[I][j][4 * q + 0], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+        }, rd, RS);
+        return;
+    }
     char *__restrict__ C = static_cast<char *>(g.c);
     constexpr int CSZ = (DT_C == MI355_DTYPE_F32) ? 4 : 2;
     const int64_t cbase = batch * g.stride_c;
@@ -756,11 +773,11 @@ gemm_lp256w4_kernel(gemm_args g)
 #endif
 }
 
-template <int DT, int DT_C, bool BNN = false, int DTB = DT, bool MX = false, bool ATN = false, int NJ = 4, int NI = 4>
-void launch(mi355_ctx *ctx, hipStream_t s, const gemm_args &g, uint32_t batch)
+template <int DT, int DT_C, bool BNN = false, int DTB = DT, bool MX = false, bool ATN = false, int NJ = 4, int NI = 4, class ARGS>
+void launch(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp256w4_kernel<DT, DT_C, BNN, DTB, MX, ATN, NJ, NI>), LDS_BYTES);
-    hipLaunchKernelGGL((gemm_lp256w4_kernel<DT, DT_C, BNN, DTB, MX, ATN, NJ, NI>), dim3(g.tiles_m * g.tiles_n, batch), dim3(256), LDS_BYTES, s, g);
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_lp256w4_kernel<DT, DT_C, BNN, DTB, MX, ATN, NJ, NI, ARGS>), LDS_BYTES);
+    hipLaunchKernelGGL((gemm_lp256w4_kernel<DT, DT_C, BNN, DTB, MX, ATN, NJ, NI, ARGS>), dim3(g.tiles_m * g.tiles_n, batch), dim3(256), LDS_BYTES, s, g);
 }
 
 }  // namespace
@@ -804,7 +821,7 @@ bool gemm_lp256w4_supports(const mi355_gemm_desc &d, const void *a, const void *
 }
 
 int32_t launch_gemm_lp256w4(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b,
-                            void *c, const void *c_in)
+                            void *c, const void *c_in, const epilogue_args *ep)
 {
     if (!gemm_lp256w4_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "lp256w4 GEMM: shape/layout not supported by this kernel");
@@ -820,40 +837,44 @@ int32_t launch_gemm_lp256w4(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc
     g.tiles_n = (uint32_t)((d.n + BN - 1) / BN);
     g.group_m = W4_GROUP_M;
     const uint32_t batch = (uint32_t)d.batch;
-    if (d.dtype_ab == MI355_DTYPE_F8E4M3) {
-        if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(ctx, s, g, batch);
-        else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(ctx, s, g, batch);
-        else launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(ctx, s, g, batch);
-    } else if (d.dtype_ab == MI355_DTYPE_F8E5M2) {
-        if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(ctx, s, g, batch);
-        else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(ctx, s, g, batch);
-        else launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(ctx, s, g, batch);
-    } else if (d.dtype_ab == MI355_DTYPE_F32) {
-        if (d.trans_b) launch<MI355_DTYPE_F32, MI355_DTYPE_F32, false>(ctx, s, g, batch);
-        else launch<MI355_DTYPE_F32, MI355_DTYPE_F32, true>(ctx, s, g, batch);
-    } else if (d.dtype_ab == MI355_DTYPE_BF16) {
-        if (d.trans_a) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true, MI355_DTYPE_BF16, false, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true, MI355_DTYPE_BF16, false, true>(ctx, s, g, batch);
-        } else if (d.trans_b) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(ctx, s, g, batch);
+    auto go = [&](const auto &g) {
+        if (d.dtype_ab == MI355_DTYPE_F8E4M3) {
+            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F32>(ctx, s, g, batch);
+            else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            else launch<MI355_DTYPE_F8E4M3, MI355_DTYPE_F16>(ctx, s, g, batch);
+        } else if (d.dtype_ab == MI355_DTYPE_F8E5M2) {
+            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F32>(ctx, s, g, batch);
+            else if (d.dtype_c == MI355_DTYPE_BF16) launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            else launch<MI355_DTYPE_F8E5M2, MI355_DTYPE_F16>(ctx, s, g, batch);
+        } else if (d.dtype_ab == MI355_DTYPE_F32) {
+            if (d.trans_b) launch<MI355_DTYPE_F32, MI355_DTYPE_F32, false>(ctx, s, g, batch);
+            else launch<MI355_DTYPE_F32, MI355_DTYPE_F32, true>(ctx, s, g, batch);
+        } else if (d.dtype_ab == MI355_DTYPE_BF16) {
+            if (d.trans_a) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true, MI355_DTYPE_BF16, false, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true, MI355_DTYPE_BF16, false, true>(ctx, s, g, batch);
+            } else if (d.trans_b) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16>(ctx, s, g, batch);
+            } else {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true>(ctx, s, g, batch);
+            }
         } else {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_BF16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_BF16, MI355_DTYPE_BF16, true>(ctx, s, g, batch);
+            if (d.trans_a) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true, MI355_DTYPE_F16, false, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true, MI355_DTYPE_F16, false, true>(ctx, s, g, batch);
+            } else if (d.trans_b) {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(ctx, s, g, batch);
+            } else {
+                if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
+                else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true>(ctx, s, g, batch);
+            }
         }
-    } else {
-        if (d.trans_a) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true, MI355_DTYPE_F16, false, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true, MI355_DTYPE_F16, false, true>(ctx, s, g, batch);
-        } else if (d.trans_b) {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16>(ctx, s, g, batch);
-        } else {
-            if (d.dtype_c == MI355_DTYPE_F32) launch<MI355_DTYPE_F16, MI355_DTYPE_F32, true>(ctx, s, g, batch);
-            else launch<MI355_DTYPE_F16, MI355_DTYPE_F16, true>(ctx, s, g, batch);
-        }
-    }
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
     check_launch(ctx, "mi355_gemm(lp256w4)");
     return MI355_OK;
 }
@@ -866,7 +887,8 @@ bool gemm_lp256x192_supports(const mi355_gemm_desc &d, const void *a, const void
     return gemm_lp256w4_supports(d, a, b, c);
 }
 
-int32_t launch_gemm_lp256x192(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, int tile_rows)
+int32_t launch_gemm_lp256x192(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, int tile_rows,
+                              const epilogue_args *ep)
 {
     if (!gemm_lp256x192_supports(d, a, b, c) || (tile_rows != 256 && tile_rows != 192))
         return fail(ctx, MI355_E_UNSUPPORTED, "lp256x192 GEMM: shape/layout not supported by this kernel");
@@ -890,8 +912,12 @@ int32_t launch_gemm_lp256x192(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_de
             else launch<HF, HF, NN, HF, false, false, 3, NI_>(ctx, s, g, batch);                                \
         }                                                                                                      \
     } while (0)
-    if (d.trans_b) { if (tile_rows == 192) X192_LAUNCH(false, 3); else X192_LAUNCH(false, 4); }
-    else { if (tile_rows == 192) X192_LAUNCH(true, 3); else X192_LAUNCH(true, 4); }
+    auto go = [&](const auto &g) {
+        if (d.trans_b) { if (tile_rows == 192) X192_LAUNCH(false, 3); else X192_LAUNCH(false, 4); }
+        else { if (tile_rows == 192) X192_LAUNCH(true, 3); else X192_LAUNCH(true, 4); }
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
 #undef X192_LAUNCH
     check_launch(ctx, "mi355_gemm(lp256x192)");
     return MI355_OK;

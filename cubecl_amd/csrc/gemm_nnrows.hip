@@ -29,7 +29,7 @@
 //
 // Accumulation: f32, order fixed by (S, slices) = by the shape and the device's CU count -- run-to-run bit-identical; not
 // bit-identical to the other kernels (different association), inside the parity tolerance of tests/test_gpu_gemm.py.
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 #include <type_traits>
 
 using namespace mi355;
@@ -114,8 +114,8 @@ template <int MB, int EB> struct nn_geom {
     static constexpr int KC = 16384 / (MB * EB);                           // k values of x per LDS chunk (64 KiB): a chunk boundary drains the ring
 };
 
-template <int DT, int MB, int S>
-__global__ void __launch_bounds__(256) gemm_nnrows_kernel(const nn_args g)
+template <int DT, int MB, int S, class ARGS = nn_args>
+__global__ void __launch_bounds__(256) gemm_nnrows_kernel(const ARGS g)
 {
     constexpr int U = NNR_U;
     typedef typename nn_elem<DT>::type ET;
@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(256) gemm_nnrows_kernel(const nn_args g)
             }
     }
     __syncthreads();
+    const epilogue_args *ep = nullptr;
+    if constexpr (has_epilogue<ARGS>) ep = &epilogue_of<ARGS>();
     const int64_t strip_col = (int64_t)strip * COLS;
     char *C = static_cast<char *>(g.c);
     const int64_t cbase = (int64_t)batch * g.stride_c;
@@ -361,7 +363,10 @@ __global__ void __launch_bounds__(256) gemm_nnrows_kernel(const nn_args g)
         for (int cp = 1; cp < NCOPY; ++cp) s += *reinterpret_cast<const f32x4 *>(red + ((cp * MP + mm) * COLS + c4));
         if (g.slices == 1) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) store_c(C, g.dtype_c, cbase + (int64_t)mm * g.ldc + strip_col + c4 + e, s[e]);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (has_epilogue<ARGS>) s[e] = finish_one(*ep, batch, mm, strip_col + c4 + e, s[e]);
+                store_c(C, g.dtype_c, cbase + (int64_t)mm * g.ldc + strip_col + c4 + e, s[e]);
+            }
         } else {                                                           // write-through (sc1) 8-byte stores: see the hand-off below
             gu64 *dst = (gu64 *)reinterpret_cast<unsigned long long *>(part + ((int64_t)slice * g.m + mm) * g.n + strip_col + c4);
             __hip_atomic_store(dst, ((unsigned long long)__float_as_uint(s[1]) << 32) | __float_as_uint(s[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -433,7 +438,10 @@ __global__ void __launch_bounds__(256) gemm_nnrows_kernel(const nn_args g)
             for (int qd = 0; qd < QD; ++qd)
                 if (live[qd]) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) store_c(C, g.dtype_c, cbase + (int64_t)mm[qd] * g.ldc + strip_col + c4[qd] + e, sum[qd][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (has_epilogue<ARGS>) sum[qd][e] = finish_one(*ep, batch, mm[qd], strip_col + c4[qd] + e, sum[qd][e]);
+                        store_c(C, g.dtype_c, cbase + (int64_t)mm[qd] * g.ldc + strip_col + c4[qd] + e, sum[qd][e]);
+                    }
                 }
         }
     };
@@ -453,24 +461,24 @@ template <int DT, int MB, int S> constexpr size_t lds_bytes()
     return x > r ? x : r;
 }
 
-template <int DT, int MB, int S>
-void launch_one(mi355_ctx *ctx, hipStream_t s, const nn_args &g, uint32_t batch)
+template <int DT, int MB, int S, class ARGS>
+void launch_one(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     constexpr size_t LDS = lds_bytes<DT, MB, S>();
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_nnrows_kernel<DT, MB, S>), LDS);
-    hipLaunchKernelGGL((gemm_nnrows_kernel<DT, MB, S>), dim3((uint32_t)(g.strips * g.slices), batch), dim3(256), LDS, s, g);
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_nnrows_kernel<DT, MB, S, ARGS>), LDS);
+    hipLaunchKernelGGL((gemm_nnrows_kernel<DT, MB, S, ARGS>), dim3((uint32_t)(g.strips * g.slices), batch), dim3(256), LDS, s, g);
 }
 
-template <int DT, int MB>
-void launch_s(mi355_ctx *ctx, hipStream_t s, const nn_args &g, uint32_t batch, int strip_bytes)
+template <int DT, int MB, class ARGS>
+void launch_s(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch, int strip_bytes)
 {
     if (strip_bytes == 1024) launch_one<DT, MB, 1024>(ctx, s, g, batch);
     else if (strip_bytes == 512) launch_one<DT, MB, 512>(ctx, s, g, batch);
     else launch_one<DT, MB, 256>(ctx, s, g, batch);
 }
 
-template <int DT>
-void launch_dt(mi355_ctx *ctx, hipStream_t s, const nn_args &g, uint32_t batch, int strip_bytes)
+template <int DT, class ARGS>
+void launch_dt(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch, int strip_bytes)
 {
     static const int min_rows_16 = [] { const char *e = getenv("MI355_NNROWS_ROWS16_FROM"); return e ? atoi(e) : 9; }();   // dev: rows from which the 16-row form runs
     if (g.m >= min_rows_16 && strip_bytes == 256) launch_s<DT, 4>(ctx, s, g, batch, strip_bytes);
@@ -571,7 +579,7 @@ bool gemm_nnrows_ready(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d)
     return it != ctx->scratch.end() && it->second.second >= (size_t)d.batch * p.slices * d.m * d.n * sizeof(float);
 }
 
-int32_t launch_gemm_nnrows(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_nnrows(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     if (!gemm_nnrows_supports(d, a, b, c))
         return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the few-rows x row-major-weight kernel does not take this descriptor");
@@ -596,9 +604,13 @@ int32_t launch_gemm_nnrows(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc 
         const int32_t rc = strip_tickets_for_stream(ctx, s, &g.tickets);
         if (rc != MI355_OK) return rc;
     }
-    if (d.dtype_ab == MI355_DTYPE_F32) launch_dt<MI355_DTYPE_F32>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
-    else if (d.dtype_ab == MI355_DTYPE_BF16) launch_dt<MI355_DTYPE_BF16>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
-    else launch_dt<MI355_DTYPE_F16>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
+    auto go = [&](const auto &g) {
+        if (d.dtype_ab == MI355_DTYPE_F32) launch_dt<MI355_DTYPE_F32>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
+        else if (d.dtype_ab == MI355_DTYPE_BF16) launch_dt<MI355_DTYPE_BF16>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
+        else launch_dt<MI355_DTYPE_F16>(ctx, s, g, (uint32_t)d.batch, p.strip_bytes);
+    };
+    if (ep) go(add_epilogue(g, *ep));
+    else go(g);
     if (p.slices > 1 && hipPeekAtLastError() != hipSuccess) strip_tickets_mark_dirty(ctx);   // a refused launch never resets its tickets
     check_launch(ctx, "mi355_gemm(nnrows)");
     return MI355_OK;

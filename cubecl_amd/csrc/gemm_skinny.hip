@@ -20,7 +20,7 @@
 //
 // Accumulation is f32 in a fixed order (K slices of a lane ascending, then the butterfly): deterministic, not bit-identical
 // to the MFMA kernels (different association), within the parity tolerance of tests/test_gpu_gemm.py.
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -102,8 +102,8 @@ __device__ __forceinline__ void store_one(void *out, int64_t idx, float v, int32
     else static_cast<uint16_t *>(out)[idx] = f32_to_f16_rne(v);
 }
 
-template <int DT, int MT, int RW>
-__global__ __launch_bounds__(WAVES * 64) void gemm_skinny_kernel(skinny_args g)
+template <int DT, int MT, int RW, class ARGS = skinny_args>
+__global__ __launch_bounds__(WAVES * 64) void gemm_skinny_kernel(ARGS g)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row0 = ((int64_t)blockIdx.x * WAVES + wave) * RW;
@@ -198,26 +198,28 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_skinny_kernel(skinny_args g)
         if (m < g.small_rows && row0 + r < g.big_rows) {
             char *out = static_cast<char *>(g.out);
             const int64_t o = (int64_t)blockIdx.y * g.stride_out + (int64_t)m * g.out_stride_small + (row0 + r) * g.out_stride_big;
+            if constexpr (has_epilogue<ARGS>) v[0] = finish_small_big(epilogue_of<ARGS>(), blockIdx.y, m, row0 + r, v[0]);
             store_one(out, o, v[0], g.dtype_c);
         }
     }
 }
 
 template <int DT, int MT, int RW>
-void launch_one(hipStream_t s, const skinny_args &g, uint32_t batch)
+void launch_one(hipStream_t s, const skinny_args &g, uint32_t batch, const epilogue_args *ep)
 {
     const dim3 grid((uint32_t)((g.big_rows + WAVES * RW - 1) / (WAVES * RW)), batch), block(WAVES * 64);
-    hipLaunchKernelGGL((gemm_skinny_kernel<DT, MT, RW>), grid, block, 0, s, g);
+    if (ep) hipLaunchKernelGGL((gemm_skinny_kernel<DT, MT, RW, with_epilogue<skinny_args>>), grid, block, 0, s, add_epilogue(g, *ep));
+    else hipLaunchKernelGGL((gemm_skinny_kernel<DT, MT, RW>), grid, block, 0, s, g);
 }
 
 template <int DT>
-void launch_dt(hipStream_t s, const skinny_args &g, uint32_t batch)
+void launch_dt(hipStream_t s, const skinny_args &g, uint32_t batch, const epilogue_args *ep)
 {
-    if (g.small_rows <= 1) launch_one<DT, 1, 1>(s, g, batch);
-    else if (g.small_rows <= 2) launch_one<DT, 2, 4>(s, g, batch);
-    else if (g.small_rows <= 4) launch_one<DT, 4, 2>(s, g, batch);
-    else if (g.small_rows <= 8) launch_one<DT, 8, 2>(s, g, batch);
-    else launch_one<DT, 16, 2>(s, g, batch);
+    if (g.small_rows <= 1) launch_one<DT, 1, 1>(s, g, batch, ep);
+    else if (g.small_rows <= 2) launch_one<DT, 2, 4>(s, g, batch, ep);
+    else if (g.small_rows <= 4) launch_one<DT, 4, 2>(s, g, batch, ep);
+    else if (g.small_rows <= 8) launch_one<DT, 8, 2>(s, g, batch, ep);
+    else launch_one<DT, 16, 2>(s, g, batch, ep);
 }
 
 }  // namespace
@@ -241,7 +243,7 @@ bool gemm_skinny_supports(const mi355_gemm_desc &d, const void *a, const void *b
     return true;
 }
 
-int32_t launch_gemm_skinny(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_skinny(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     if (!gemm_skinny_supports(d, a, b, c)) return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the skinny kernel does not take this descriptor");
     skinny_args g{};
@@ -260,9 +262,12 @@ int32_t launch_gemm_skinny(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc 
     g.big_rows = (int32_t)(a_small ? d.n : d.m);
     g.k = (int32_t)d.k;
     g.dtype_c = d.dtype_c;
-    if (d.dtype_ab == MI355_DTYPE_F32) launch_dt<MI355_DTYPE_F32>(s, g, (uint32_t)d.batch);
-    else if (d.dtype_ab == MI355_DTYPE_BF16) launch_dt<MI355_DTYPE_BF16>(s, g, (uint32_t)d.batch);
-    else launch_dt<MI355_DTYPE_F16>(s, g, (uint32_t)d.batch);
+    epilogue_args e;
+    const epilogue_args *pe = nullptr;
+    if (ep) { e = *ep; e.swapped = !a_small; pe = &e; }
+    if (d.dtype_ab == MI355_DTYPE_F32) launch_dt<MI355_DTYPE_F32>(s, g, (uint32_t)d.batch, pe);
+    else if (d.dtype_ab == MI355_DTYPE_BF16) launch_dt<MI355_DTYPE_BF16>(s, g, (uint32_t)d.batch, pe);
+    else launch_dt<MI355_DTYPE_F16>(s, g, (uint32_t)d.batch, pe);
     check_launch(ctx, "mi355_gemm(skinny)");
     return MI355_OK;
 }

@@ -29,7 +29,7 @@
 #include <algorithm>
 #include <cstdlib>
 
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -176,8 +176,8 @@ template <int MB, bool TWO, int NB = 1> struct ring_geom {
 // streamed operand as of the small one, so the ring keeps 80 KiB of it in flight where the NB = 1 form had 48 (measured bound of
 // that form: ~4.1 TB/s whatever the HBM side did, profiles/r03_stream64_cold_ablation.txt).  The price is the slices' meeting
 // in memory: f32 blocks + one ticket per row block, folded in slice order by the last workgroup to arrive (as gemm_nnrows.hip).
-template <int DT, int MB, bool TWO, int NB = 1>
-__global__ void __launch_bounds__(512 + 64 * NLB, TWO ? (NLB == 2 ? 5 : 6) : (NLB == 2 ? 2 : 3)) gemm_stream64_kernel(stream_args g)
+template <int DT, int MB, bool TWO, int NB = 1, class ARGS = stream_args>
+__global__ void __launch_bounds__(512 + 64 * NLB, TWO ? (NLB == 2 ? 5 : 6) : (NLB == 2 ? 2 : 3)) gemm_stream64_kernel(ARGS g)
 {
     // Two rings.  The streamed operand needs DEPTH: ~25 GB/s per CU x ~2.5 us of HBM latency under load = ~64 KiB in flight
     // (with both operands in one 12-16 slot ring only 40-48 KiB of it were, and the kernel sat at 4.5 TB/s).  The small
@@ -371,7 +371,10 @@ __global__ void __launch_bounds__(512 + 64 * NLB, TWO ? (NLB == 2 ? 5 : 6) : (NL
         for (int ww = 1; ww < 4; ++ww) v += part[((ww * NB * MB + blk) * 32 + row) * PP + col];
         return v;
     };
+    const epilogue_args *ep = nullptr;
+    if constexpr (has_epilogue<ARGS>) ep = &epilogue_of<ARGS>();
     auto store_out = [&](int64_t sm, int64_t bg, float v) {
+        if constexpr (has_epilogue<ARGS>) v = finish_small_big(*ep, blockIdx.y, sm, bg, v);
         const int64_t o = (int64_t)blockIdx.y * g.stride_out + sm * g.out_stride_small + bg * g.out_stride_big;
         if (g.dtype_c == MI355_DTYPE_F32) reinterpret_cast<float *>(out)[o] = v;
         else if (g.dtype_c == MI355_DTYPE_BF16) reinterpret_cast<uint16_t *>(out)[o] = f32_to_bf16_rne(v);
@@ -434,31 +437,38 @@ __global__ void __launch_bounds__(512 + 64 * NLB, TWO ? (NLB == 2 ? 5 : 6) : (NL
     }
 }
 
-template <int DT, int MB, bool TWO>
-void launch_form(mi355_ctx *ctx, hipStream_t s, const stream_args &g, uint32_t batch)
+template <int DT, int MB, bool TWO, class ARGS>
+void launch_form(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     constexpr int LDS = ring_geom<MB, TWO>::LDS;
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_kernel<DT, MB, TWO>), LDS);
-    hipLaunchKernelGGL((gemm_stream64_kernel<DT, MB, TWO>), dim3((uint32_t)((g.big_rows + BN - 1) / BN), batch), dim3(512 + 64 * NLB), LDS, s, g);
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_kernel<DT, MB, TWO, 1, ARGS>), LDS);
+    hipLaunchKernelGGL((gemm_stream64_kernel<DT, MB, TWO, 1, ARGS>), dim3((uint32_t)((g.big_rows + BN - 1) / BN), batch), dim3(512 + 64 * NLB), LDS, s, g);
 }
 
 // the NB = 2 form: 64 streamed rows per workgroup, K in g.slices slices (one workgroup per CU: the deep rings)
-template <int DT, int MB>
-void launch_wide(mi355_ctx *ctx, hipStream_t s, const stream_args &g, uint32_t batch)
+template <int DT, int MB, class ARGS>
+void launch_wide(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     constexpr int LDS = ring_geom<MB, false, 2>::LDS;
-    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_kernel<DT, MB, false, 2>), LDS);
+    lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_kernel<DT, MB, false, 2, ARGS>), LDS);
     const uint32_t nblocks = (uint32_t)((g.big_rows + 2 * BN - 1) / (2 * BN));
-    hipLaunchKernelGGL((gemm_stream64_kernel<DT, MB, false, 2>), dim3(nblocks * (uint32_t)g.slices, batch), dim3(512 + 64 * NLB), LDS, s, g);
+    hipLaunchKernelGGL((gemm_stream64_kernel<DT, MB, false, 2, ARGS>), dim3(nblocks * (uint32_t)g.slices, batch), dim3(512 + 64 * NLB), LDS, s, g);
 }
 
-template <int DT, int MB>
-void launch_one(mi355_ctx *ctx, hipStream_t s, const stream_args &g, uint32_t batch)
+template <int DT, int MB, class ARGS>
+void launch_args(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     if (g.slices > 1) return launch_wide<DT, MB>(ctx, s, g, batch);
     const uint64_t wgs = (uint64_t)((g.big_rows + BN - 1) / BN) * batch;
     if (wgs > (uint64_t)ctx->props.num_streaming_multiprocessors) launch_form<DT, MB, true>(ctx, s, g, batch);
     else launch_form<DT, MB, false>(ctx, s, g, batch);
+}
+
+template <int DT, int MB>
+void launch_one(mi355_ctx *ctx, hipStream_t s, const stream_args &g, uint32_t batch, const epilogue_args *ep)
+{
+    if (ep) launch_args<DT, MB>(ctx, s, add_epilogue(g, *ep), batch);
+    else launch_args<DT, MB>(ctx, s, g, batch);
 }
 
 }  // namespace
@@ -504,9 +514,9 @@ bool gemm_stream64_supports(const mi355_gemm_desc &d, const void *a, const void 
     return true;
 }
 
-int32_t launch_gemm_stream64(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_stream64(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
-    if (d.dtype_ab == MI355_DTYPE_F32) return launch_gemm_stream64_f32(ctx, s, d, a, b, c);
+    if (d.dtype_ab == MI355_DTYPE_F32) return launch_gemm_stream64_f32(ctx, s, d, a, b, c, ep);
     if (!gemm_stream64_supports(d, a, b, c)) return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the 64-row streaming kernel does not take this descriptor");
     stream_args g{};
     const bool a_small = d.m <= d.n;
@@ -543,12 +553,15 @@ int32_t launch_gemm_stream64(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_des
         else g.slices = 0;
     }
     if (g.slices <= 1) g.slices = 1;
+    epilogue_args e;
+    const epilogue_args *pe = nullptr;
+    if (ep) { e = *ep; e.swapped = !a_small; pe = &e; }
     if (d.dtype_ab == MI355_DTYPE_BF16) {
-        if (two) launch_one<MI355_DTYPE_BF16, 2>(ctx, s, g, batch);
-        else launch_one<MI355_DTYPE_BF16, 1>(ctx, s, g, batch);
+        if (two) launch_one<MI355_DTYPE_BF16, 2>(ctx, s, g, batch, pe);
+        else launch_one<MI355_DTYPE_BF16, 1>(ctx, s, g, batch, pe);
     } else {
-        if (two) launch_one<MI355_DTYPE_F16, 2>(ctx, s, g, batch);
-        else launch_one<MI355_DTYPE_F16, 1>(ctx, s, g, batch);
+        if (two) launch_one<MI355_DTYPE_F16, 2>(ctx, s, g, batch, pe);
+        else launch_one<MI355_DTYPE_F16, 1>(ctx, s, g, batch, pe);
     }
     if (g.slices > 1 && hipPeekAtLastError() != hipSuccess) strip_tickets_mark_dirty(ctx);   // a refused launch never resets its tickets
     check_launch(ctx, "mi355_gemm(stream64)");

@@ -26,7 +26,7 @@
 #include <cstdlib>
 #include <type_traits>
 
-#include "gemm_common.hpp"
+#include "gemm_epilogue.hpp"
 
 using namespace mi355;
 
@@ -82,8 +82,8 @@ template <int N> __device__ __forceinline__ void wait_vmcnt()
 
 // MB: 16-row blocks of the small operand; NBW: 16-row blocks of the streamed operand per workgroup; S: ring stages per wave;
 // NT: the streamed operand cannot stay in the Infinity Cache anyway -- non-temporal pieces (as gemm_stream64.hip)
-template <int MB, int NBW, int S, bool NT>
-__global__ __launch_bounds__(WAVES * 64) void gemm_stream64_f32_kernel(rows_args g)
+template <int MB, int NBW, int S, bool NT, class ARGS = rows_args>
+__global__ __launch_bounds__(WAVES * 64) void gemm_stream64_f32_kernel(ARGS g)
 {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int BLOCKS = NBW + MB, STAGE_BYTES = BLOCKS * BLOCK_BYTES, PIECES = 4 * BLOCKS;   // DMA pieces of one stage
@@ -209,7 +209,9 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_stream64_f32_kernel(rows_args
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int m = 16 * a + 4 * gq + r;
-            if (m < g.small_rows) out[(int64_t)m * g.out_stride_small] = sum[r];
+            if (m >= g.small_rows) continue;
+            if constexpr (has_epilogue<ARGS>) out[(int64_t)m * g.out_stride_small] = finish_small_big(epilogue_of<ARGS>(), blockIdx.y, m, n, sum[r]);
+            else out[(int64_t)m * g.out_stride_small] = sum[r];
         }
     }
 }
@@ -222,8 +224,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_stream64_f32_kernel(rows_args
 // the streamed operand in flight.  No K split, so no final fold.  The bound is the f32 matrix core: 32 MFMAs x 32 cycles per wave
 // and K-block of 64 -- 131 k cycles = 62 us at 64 x 8192 x 8192 (measured: 97.5, against 106.1 on the K-split form; the refill's DMA pieces are
 // dealt out among the MFMAs in both forms: issued as a block in front of them they cost 64 rows 15 us).
-template <int MB, int S, bool NT>
-__global__ __launch_bounds__(MB * 64) void gemm_stream64_f32_rows_kernel(rows_args g)
+template <int MB, int S, bool NT, class ARGS = rows_args>
+__global__ __launch_bounds__(MB * 64) void gemm_stream64_f32_rows_kernel(ARGS g)
 {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int NBW = 2, STAGE_BYTES = (NBW + MB) * BLOCK_BYTES, WSHARE = (NBW * 4 + MB - 1) / MB, PIECES = 4 + WSHARE;
@@ -321,38 +323,40 @@ __global__ __launch_bounds__(MB * 64) void gemm_stream64_f32_rows_kernel(rows_ar
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int m = 16 * wave + 4 * gq + r;
-            if (m < g.small_rows) out[(int64_t)m * g.out_stride_small] = sum[r];
+            if (m >= g.small_rows) continue;
+            if constexpr (has_epilogue<ARGS>) out[(int64_t)m * g.out_stride_small] = finish_small_big(epilogue_of<ARGS>(), blockIdx.y, m, n, sum[r]);
+            else out[(int64_t)m * g.out_stride_small] = sum[r];
         }
     }
 }
 
-template <int MB, int S>
-void launch_rows_form(mi355_ctx *ctx, hipStream_t s, const rows_args &g, uint32_t batch)
+template <int MB, int S, class ARGS>
+void launch_rows_form(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     constexpr int LDS = S * (2 + MB) * BLOCK_BYTES;
     const uint32_t nblocks = (uint32_t)((g.big_rows + 31) / 32);
     if ((int64_t)g.big_rows * g.k * 4 * batch > (192ll << 20)) {
-        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_rows_kernel<MB, S, true>), LDS);
-        hipLaunchKernelGGL((gemm_stream64_f32_rows_kernel<MB, S, true>), dim3(nblocks, batch), dim3(MB * 64), LDS, s, g);
+        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_rows_kernel<MB, S, true, ARGS>), LDS);
+        hipLaunchKernelGGL((gemm_stream64_f32_rows_kernel<MB, S, true, ARGS>), dim3(nblocks, batch), dim3(MB * 64), LDS, s, g);
     } else {
-        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_rows_kernel<MB, S, false>), LDS);
-        hipLaunchKernelGGL((gemm_stream64_f32_rows_kernel<MB, S, false>), dim3(nblocks, batch), dim3(MB * 64), LDS, s, g);
+        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_rows_kernel<MB, S, false, ARGS>), LDS);
+        hipLaunchKernelGGL((gemm_stream64_f32_rows_kernel<MB, S, false, ARGS>), dim3(nblocks, batch), dim3(MB * 64), LDS, s, g);
     }
 }
 
-template <int MB, int NBW, int S>
-void launch_form(mi355_ctx *ctx, hipStream_t s, const rows_args &g, uint32_t batch)
+template <int MB, int NBW, int S, class ARGS>
+void launch_form(mi355_ctx *ctx, hipStream_t s, const ARGS &g, uint32_t batch)
 {
     constexpr int LDS = WAVES * S * (NBW + MB) * BLOCK_BYTES;
     static_assert(LDS <= 160 * 1024 && LDS >= WAVES * MB * NBW * 1024, "rings fit the CU's LDS and hold the final fold");
     const uint32_t nblocks = (uint32_t)((g.big_rows + 16 * NBW - 1) / (16 * NBW));
     // streamed bytes of the whole launch against what the 256 MiB Infinity Cache could still hold next to everything else
     if ((int64_t)g.big_rows * g.k * 4 * batch > (192ll << 20)) {
-        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_kernel<MB, NBW, S, true>), LDS);
-        hipLaunchKernelGGL((gemm_stream64_f32_kernel<MB, NBW, S, true>), dim3(nblocks, batch), dim3(WAVES * 64), LDS, s, g);
+        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_kernel<MB, NBW, S, true, ARGS>), LDS);
+        hipLaunchKernelGGL((gemm_stream64_f32_kernel<MB, NBW, S, true, ARGS>), dim3(nblocks, batch), dim3(WAVES * 64), LDS, s, g);
     } else {
-        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_kernel<MB, NBW, S, false>), LDS);
-        hipLaunchKernelGGL((gemm_stream64_f32_kernel<MB, NBW, S, false>), dim3(nblocks, batch), dim3(WAVES * 64), LDS, s, g);
+        lds_opt_in(ctx, reinterpret_cast<const void *>(gemm_stream64_f32_kernel<MB, NBW, S, false, ARGS>), LDS);
+        hipLaunchKernelGGL((gemm_stream64_f32_kernel<MB, NBW, S, false, ARGS>), dim3(nblocks, batch), dim3(WAVES * 64), LDS, s, g);
     }
 }
 
@@ -404,7 +408,7 @@ bool stream64_f32_rows_form(const mi355_gemm_desc &d, int cus)
     return wgs >= cus && wgs <= 2 * cus;
 }
 
-int32_t launch_gemm_stream64_f32(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c)
+int32_t launch_gemm_stream64_f32(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     if (!gemm_stream64_f32_supports(d, a, b, c)) return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the f32 streaming kernel does not take this descriptor");
     rows_args g{};
@@ -425,15 +429,22 @@ int32_t launch_gemm_stream64_f32(mi355_ctx *ctx, hipStream_t s, const mi355_gemm
     const uint32_t batch = (uint32_t)d.batch;
     const int cus = ctx->props.num_streaming_multiprocessors > 0 ? ctx->props.num_streaming_multiprocessors : 256;
     const int nbw = stream64_f32_blocks(d, cus);
-    if (g.small_rows <= 16) {
-        if (nbw == 2) launch_form<1, 2, 3>(ctx, s, g, batch);
-        else launch_form<1, 1, 4>(ctx, s, g, batch);
-    } else if (g.small_rows <= 32) {
-        if (nbw == 2) launch_form<2, 2, 2>(ctx, s, g, batch);
-        else launch_form<2, 1, 3>(ctx, s, g, batch);
-    } else if (g.small_rows <= 48) launch_form<3, 1, 2>(ctx, s, g, batch);
-    else if (stream64_f32_rows_form(d, cus)) launch_rows_form<4, 6>(ctx, s, g, batch);
-    else launch_form<4, 1, 2>(ctx, s, g, batch);
+    auto go = [&](const auto &g) {
+        if (g.small_rows <= 16) {
+            if (nbw == 2) launch_form<1, 2, 3>(ctx, s, g, batch);
+            else launch_form<1, 1, 4>(ctx, s, g, batch);
+        } else if (g.small_rows <= 32) {
+            if (nbw == 2) launch_form<2, 2, 2>(ctx, s, g, batch);
+            else launch_form<2, 1, 3>(ctx, s, g, batch);
+        } else if (g.small_rows <= 48) launch_form<3, 1, 2>(ctx, s, g, batch);
+        else if (stream64_f32_rows_form(d, cus)) launch_rows_form<4, 6>(ctx, s, g, batch);
+        else launch_form<4, 1, 2>(ctx, s, g, batch);
+    };
+    if (ep) {
+        with_epilogue<rows_args> w = add_epilogue(g, *ep);
+        w.ep.swapped = !a_small;
+        go(w);
+    } else go(g);
     check_launch(ctx, "mi355_gemm(stream64, f32)");
     return MI355_OK;
 }

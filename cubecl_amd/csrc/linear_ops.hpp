@@ -44,15 +44,22 @@ inline row_shape shape_for(int64_t rows, int64_t cols)
     return {1024, 2};
 }
 
+// The gradient keeps the weight and its gradient in registers too: its longest rows take half the threads with twice the registers each.
+inline row_shape grad_shape_for(int64_t rows, int64_t cols)
+{
+    const row_shape sh = shape_for(rows, cols);
+    return sh.threads == 1024 && sh.pieces == 2 ? row_shape{512, 4} : sh;
+}
+
 // workgroups of the gradient: each walks rows / grid of them and leaves one partial row (four, T = 64) of the weight's gradient
 constexpr int64_t GRAD_WGS = 512, LONG_SLABS = 64;
 inline int64_t norm_grad_wgs(int64_t rows, const row_shape &sh)
 {
-    return std::min(sh.threads == 64 ? (rows + 3) / 4 : rows, sh.threads == 1024 ? GRAD_WGS / 2 : GRAD_WGS);
+    return std::min(sh.threads == 64 ? (rows + 3) / 4 : rows, sh.threads >= 512 ? GRAD_WGS / 2 : GRAD_WGS);
 }
 inline int64_t norm_grad_partials(int64_t rows, int64_t cols)
 {
-    const row_shape sh = shape_for(rows, cols);
+    const row_shape sh = grad_shape_for(rows, cols);
     if (sh.threads == 0) return std::min(rows, LONG_SLABS);
     return norm_grad_wgs(rows, sh) * (sh.threads == 64 ? 4 : 1);
 }
@@ -62,11 +69,44 @@ void launch_rms_norm_grad(hipStream_t s, int32_t dtype, const norm_grad_args &a)
 // column sums of f32 partial rows, [batch][count][cols] -> out [batch][cols] in `dtype`; count 0: zeros
 void launch_fold_columns(hipStream_t s, const float *partial, int64_t count, int64_t cols, int64_t batch, void *out, int32_t dtype);
 
-// ---- gemm_epilogue.hip
+// ---- the epilogue of mi355_gemm_fused: gemm_epilogue.hpp inside the GEMM kernels, gemm_epilogue.hip as a pass over a product
+constexpr float GELU_C0 = 0.797884560802865356f, GELU_C1 = 0.044715f;    // sqrt(2 / pi) and the cubic term of gelu's tanh form
+enum { ACT_LINEAR = 0, ACT_SIGMOID = 1, ACT_ERF = 2 };                   // rowops.hpp
+struct epilogue_args {
+    mi355_gemm_epilogue p;
+    float a, b, floor;
+    int32_t kind, dtype_c;
+    int32_t swapped;          // a kernel that calls its operands small and large: the small one is B
+};
+inline epilogue_args make_epilogue(const mi355_gemm_epilogue &ep, int32_t dtype_c)
+{
+    constexpr float LOG2E = 1.44269504088896340736f;
+    epilogue_args e{};
+    e.p = ep;
+    e.dtype_c = dtype_c;
+    e.floor = ep.activation == MI355_ACT_RELU ? 0.0f : -__builtin_inff();
+    e.kind = ep.activation == MI355_ACT_SILU || ep.activation == MI355_ACT_GELU_TANH ? ACT_SIGMOID : ep.activation == MI355_ACT_GELU ? ACT_ERF : ACT_LINEAR;
+    e.a = ep.activation == MI355_ACT_SILU ? -LOG2E : -2.0f * GELU_C0 * LOG2E;
+    e.b = ep.activation == MI355_ACT_SILU ? 0.0f : -2.0f * GELU_C0 * GELU_C1 * LOG2E;
+    return e;
+}
+// the same for the part of the output that begins at (row, col)
+inline epilogue_args epilogue_at(epilogue_args e, int64_t row, int64_t col)
+{
+    const int64_t ec = (int64_t)dtype_size(e.dtype_c);
+    auto by = [](const void *p, int64_t bytes) { return p ? static_cast<const char *>(p) + bytes : nullptr; };
+    if (e.p.bias) e.p.bias = by(e.p.bias, col * (int64_t)dtype_size(e.p.dtype_bias));
+    e.p.residual = by(e.p.residual, (row * e.p.ld_residual + col) * ec);
+    e.p.pre = const_cast<void *>(static_cast<const void *>(by(e.p.pre, (row * e.p.ld_pre + col) * ec)));
+    if (e.p.row_scale) e.p.row_scale += row * e.p.inc_row_scale;
+    if (e.p.col_scale) e.p.col_scale += col * e.p.inc_col_scale;
+    return e;
+}
 // what mi355_gemm_fused refuses of an epilogue (linear_ops.cpp); `d` has been validated and is not empty
 int32_t validate_epilogue(mi355_ctx *ctx, const mi355_gemm_desc &d, const mi355_gemm_epilogue &ep, const void *a, const void *b, const void *c);
-void launch_epilogue(hipStream_t s, const float *prod, const mi355_gemm_epilogue &ep, void *c, int64_t batch, int64_t m, int64_t n, int32_t dtype_c,
-                     int64_t ldc, int64_t stride_c);
+// c = the epilogue of the sum of `slabs` f32 products, slab_stride elements apart, [batch][m][n] each, added in order
+void launch_epilogue(hipStream_t s, const float *prod, uint32_t slabs, int64_t slab_stride, const epilogue_args &ep, void *c, int64_t batch, int64_t m,
+                     int64_t n, int64_t ldc, int64_t stride_c);
 struct fused_grad_args {
     const void *grad_out, *pre;
     void *grad_pre;

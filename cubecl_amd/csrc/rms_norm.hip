@@ -470,7 +470,7 @@ void launch_norm(hipStream_t s, const norm_args &a)
 template <int DT>
 void launch_norm_grad(hipStream_t s, const norm_grad_args &a)
 {
-    const row_shape sh = shape_for(a.rows, a.cols);
+    const row_shape sh = grad_shape_for(a.rows, a.cols);
     if (sh.threads == 0) {
         // (the weight's gradient first: grad_in may be one of the operands it reads)
         if (a.partial)
@@ -481,7 +481,7 @@ void launch_norm_grad(hipStream_t s, const norm_grad_args &a)
     const dim3 grid((uint32_t)norm_grad_wgs(a.rows, sh));
 #define GRAD(T, CH) else if (sh.threads == T && sh.pieces == CH) hipLaunchKernelGGL((rms_norm_grad_kernel<DT, T, CH>), grid, dim3(T < 256 ? 256 : T), 0, s, a)
     if (false) {}
-    GRAD(64, 1); GRAD(64, 2); GRAD(256, 1); GRAD(256, 2); GRAD(256, 4); GRAD(1024, 1); GRAD(1024, 2);
+    GRAD(64, 1); GRAD(64, 2); GRAD(256, 1); GRAD(256, 2); GRAD(256, 4); GRAD(512, 4); GRAD(1024, 1);
 #undef GRAD
 }
 

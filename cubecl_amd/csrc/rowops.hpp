@@ -68,16 +68,23 @@ __device__ __forceinline__ float get(const vec8<DT> &r, int e)      // e a compi
     }
 }
 
-template <int DT>
+template <bool NT, class V>
+__device__ __forceinline__ void put(V *p, const V &v)
+{
+    if constexpr (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+// NT: past the caches, for outputs larger than they are
+template <int DT, bool NT = false>
 __device__ __forceinline__ void store8(void *p, int64_t i, int valid, const float (&f)[8])
 {
     if constexpr (DT == MI355_DTYPE_F32) {
         float *q = static_cast<float *>(p) + i;
         if (valid >= 8) {
-            const u32x4 lo = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
-            const u32x4 hi = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
-            *reinterpret_cast<u32x4_e4 *>(q) = lo;
-            *reinterpret_cast<u32x4_e4 *>(q + 4) = hi;
+            const u32x4_e4 lo = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+            const u32x4_e4 hi = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+            put<NT>(reinterpret_cast<u32x4_e4 *>(q), lo);
+            put<NT>(reinterpret_cast<u32x4_e4 *>(q + 4), hi);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -86,8 +93,8 @@ __device__ __forceinline__ void store8(void *p, int64_t i, int valid, const floa
     } else {
         uint16_t *q = static_cast<uint16_t *>(p) + i;
         if (valid >= 8) {
-            const u32x4 v = {f32x2_to_lp<DT>(f[0], f[1]), f32x2_to_lp<DT>(f[2], f[3]), f32x2_to_lp<DT>(f[4], f[5]), f32x2_to_lp<DT>(f[6], f[7])};
-            *reinterpret_cast<u32x4_e2 *>(q) = v;
+            const u32x4_e2 v = {f32x2_to_lp<DT>(f[0], f[1]), f32x2_to_lp<DT>(f[2], f[3]), f32x2_to_lp<DT>(f[4], f[5]), f32x2_to_lp<DT>(f[6], f[7])};
+            put<NT>(reinterpret_cast<u32x4_e2 *>(q), v);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -183,22 +190,21 @@ __device__ __forceinline__ float erfc_abs(float x, float exp_neg_x2)
 // z limited to [lo, hi]; a NaN stays
 __device__ __forceinline__ float limit(float z, float lo, float hi) { return z < lo ? lo : (z > hi ? hi : z); }
 
-constexpr float GELU_C0 = 0.797884560802865356f, GELU_C1 = 0.044715f;    // sqrt(2 / pi) and the cubic term of gelu's tanh form
-
-template <int ACT>
-__device__ __forceinline__ float act_of(float z)
+// Five activations in three forms, so that a kernel carries three pieces of code (their constants travel in epilogue_args):
+//   linear    z, or 0 below `floor` (0: relu; -inf: none)
+//   sigmoid   z sigmoid(z (p + q z^2)): silu, and gelu's tanh form, whose (1 + tanh u) / 2 is sigmoid(2 u); a, b = -p, -q times log2(e)
+//   erf       z Phi(z)
+// At -inf the factor is 0 and the limit is 0: the multiplicand is kept finite (a NaN comes back through the factor), and so is the square (b may be 0).
+__device__ __forceinline__ float act_linear(float z, float floor) { return z < floor ? 0.0f : z; }
+__device__ __forceinline__ float act_sigmoid(float z, float a, float b)
 {
-    if constexpr (ACT == MI355_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if constexpr (ACT == MI355_ACT_NONE) return z;
-    z = z < -FLT_MAX ? -FLT_MAX : z;                            // -inf * 0 below would be NaN where the limit is 0
-    if constexpr (ACT == MI355_ACT_SILU) return z * sigmoid_of(z);
-    if constexpr (ACT == MI355_ACT_GELU_TANH) return z * sigmoid_of(2.0f * GELU_C0 * z * (1.0f + GELU_C1 * z * z));   // (1 + tanh u) / 2 = sigmoid(2 u)
-    if constexpr (ACT == MI355_ACT_GELU) {
-        const float x = fabsf(z) * 0.707106781186547524f;
-        const float q = 0.5f * erfc_abs(x, exp_of(-x * x));
-        return z * (z < 0.0f ? q : 1.0f - q);
-    }
-    return z;
+    return fmaxf(z, -FLT_MAX) * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (a + b * fminf(z * z, 1e30f))));
+}
+__device__ __forceinline__ float act_erf(float z)
+{
+    const float x = fabsf(z) * 0.707106781186547524f;
+    const float q = 0.5f * erfc_abs(x, exp_of(-x * x));
+    return fmaxf(z, -FLT_MAX) * (z < 0.0f ? q : 1.0f - q);
 }
 
 // The derivative.  Beyond the limits it is 0 or 1 to the last bit of f32; inside them nothing overflows.

@@ -11,6 +11,7 @@ reduce_matrix for sums).  These functions take exactly that contract and forward
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional
 
 from . import _native as N
@@ -20,6 +21,9 @@ from .tensor import TensorHandle, matrix_batch_layout
 
 def _matrix_operand(t: TensorHandle, name: str):
     """-> (transposed, leading dimension, batch count, batch stride)."""
+    if len(t.shape) == 2 and min(t.shape) > 1 and min(t.strides) == 1:     # one matrix, either way round: nothing to classify
+        rs, cs = t.strides
+        return (False, rs, 1, 0) if cs == 1 else (True, cs, 1, 0)
     if t.rank() < 2:
         raise ServerError(N.E_INVALID_ARGUMENT, f"matmul: {name} must have rank >= 2")
     if t.shape[-2] == 0 or t.shape[-1] == 0:   # empty operand (K == 0 or empty output): nothing is read
@@ -487,15 +491,15 @@ def _activation(name, what: str) -> int:
     return _ACTIVATIONS[name]
 
 
-def _ptr(t: Optional[TensorHandle]):
-    return C.c_void_p(t.device_ptr()) if t is not None else None
+def _ptr(t):
+    return None if t is None else t.device_ptr()
 
 
 def _batched(t: TensorHandle, tail: int, batch: int, what: str):
     """(elements between batch entries, 0 for one that all entries share) of a [.., tail] operand that goes with `batch` matrices."""
-    lead = 1
-    for d in t.shape[:t.rank() - tail]:
-        lead *= d
+    if len(t.shape) == tail:
+        return 0
+    lead = math.prod(t.shape[:t.rank() - tail])
     if lead == 1:
         return 0
     if lead != batch:
@@ -509,6 +513,8 @@ def _batched(t: TensorHandle, tail: int, batch: int, what: str):
 
 def _vector(client: ComputeClient, t: TensorHandle, n: int, batch: int, what: str):
     """-> (tensor, element stride, batch stride) of a per-row or per-column operand: [n] or [batch.., n], or one value for all."""
+    if t.shape == (n,) and n > 1 and t.strides[0] >= 0:
+        return t, t.strides[0], 0
     if t.num_elems() == 1:
         return t, 0, 0
     if t.shape[-1] != n:
@@ -560,9 +566,7 @@ def matmul_fused(client: ComputeClient, lhs: TensorHandle, rhs: TensorHandle, ou
             raise ServerError(N.E_INVALID_ARGUMENT, f"matmul_fused: {name} must be f32")
     lhs, (ta, lda, ba, sa) = _kernel_ready(client, lhs, "lhs")
     rhs, (tb, ldb, bb, sb) = _kernel_ready(client, rhs, "rhs")
-    batch = 1
-    for d in out.shape[:-2]:
-        batch *= d
+    batch = math.prod(out.shape[:-2])
     if out.num_elems() == 0:
         return
     ldc, sc = _rows_of_matrix(out, batch, "matmul_fused: out")
@@ -600,14 +604,7 @@ def matmul_fused(client: ComputeClient, lhs: TensorHandle, rhs: TensorHandle, ou
                       stride_c=sc, dtype_ab=int(lhs.dtype), dtype_c=int(out.dtype), trans_a=int(ta), trans_b=int(tb), algo=algo)
     client._s.check(client.lib.mi355_gemm_fused(
         client.ctx, client.on(lhs, rhs, out, bias, residual, lhs_scale, rhs_scale, pre_activation), C.byref(desc), C.byref(ep),
-        C.c_void_p(lhs.device_ptr()), C.c_void_p(rhs.device_ptr()), C.c_void_p(out.device_ptr())))
-
-
-def gemm_fused_plan(client: ComputeClient, desc: N.GemmDesc) -> bool:
-    """Does mi355_gemm_fused run `desc`'s epilogue inside the product's kernel (host-side only)?"""
-    fused = C.c_int32()
-    client._s.check(client.lib.mi355_gemm_fused_plan(C.byref(desc), C.byref(fused)))
-    return bool(fused.value)
+        lhs.device_ptr(), rhs.device_ptr(), out.device_ptr()))
 
 
 def _swap_last(t: TensorHandle) -> TensorHandle:
@@ -618,9 +615,7 @@ def _as_rows(client: ComputeClient, t: TensorHandle) -> TensorHandle:
     """[batch.., rows, cols] as one [batch * rows, cols] matrix, copied only where the batch does not follow on from the rows."""
     if t.rank() == 2:
         return t
-    rows, cols = 1, t.shape[-1]
-    for d in t.shape[:-1]:
-        rows *= d
+    rows, cols = math.prod(t.shape[:-1]), t.shape[-1]
     acc, fits = t.strides[-2], True
     for i in range(t.rank() - 3, -1, -1):
         acc *= t.shape[i + 1]
@@ -647,9 +642,7 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
     if grad_out.rank() < 2:
         raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_out must have rank >= 2")
     m, n = grad_out.shape[-2:]
-    batch = 1
-    for d in grad_out.shape[:-2]:
-        batch *= d
+    batch = math.prod(grad_out.shape[:-2])
     for t, name in ((pre_activation, "pre_activation"), (grad_pre, "grad_pre")):
         if t is not None and (tuple(t.shape) != tuple(grad_out.shape) or t.dtype != grad_out.dtype):
             raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: {name} must have grad_out's shape and dtype")
@@ -703,7 +696,7 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
         if need.value:
             ws = client.empty(need.value)
     client._s.check(client.lib.mi355_gemm_fused_grad(
-        client.ctx, client.on(g, z, grad_pre, grad_bias, ws), C.byref(desc), C.c_void_p(g.device_ptr()), _ptr(z), _ptr(grad_pre), _ptr(grad_bias),
+        client.ctx, client.on(g, z, grad_pre, grad_bias, ws), C.byref(desc), g.device_ptr(), _ptr(z), _ptr(grad_pre), _ptr(grad_bias),
         _ptr(ws), need.value))
     if grad_lhs is not None:
         lead = grad_lhs.num_elems() // (m * grad_lhs.shape[-1]) if grad_lhs.num_elems() else batch
@@ -748,20 +741,19 @@ def _sum_of_products(client: ComputeClient, pairs, out: TensorHandle) -> None:
         matmul(client, a, b, total, acc=total if i else None)
     if out.dtype != ElemType.F32:
         rounded = TensorHandle.new_contiguous(out.shape, client.empty(out.num_elems() * out.dtype.size()), out.dtype)
-        client._s.check(client.lib.mi355_cast(client.ctx, client.on(total, rounded), C.c_void_p(total.device_ptr()), int(ElemType.F32),
-                                              C.c_void_p(rounded.device_ptr()), int(out.dtype), out.num_elems()))
+        client._s.check(client.lib.mi355_cast(client.ctx, client.on(total, rounded), total.device_ptr(), int(ElemType.F32),
+                                              rounded.device_ptr(), int(out.dtype), out.num_elems()))
         total = rounded
     copy_into(client, total, out)
 
 
 def _norm_rows(t: TensorHandle, what: str):
     """(rows, cols, row stride) of a tensor whose last axis is the norm's; E_UNSUPPORTED_STRIDES where the rows do not collapse."""
+    if len(t.shape) == 2 and t.strides[1] == 1 and t.strides[0] >= t.shape[1] > 0:
+        return t.shape[0], t.shape[1], t.strides[0]
     if t.rank() == 0:
         raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: rank-0 tensor")
-    cols = t.shape[-1]
-    rows = 1
-    for d in t.shape[:-1]:
-        rows *= d
+    cols, rows = t.shape[-1], math.prod(t.shape[:-1])
     if rows == 0 or cols == 0:
         return rows, cols, cols
     if cols > 1 and t.strides[-1] != 1:
@@ -782,13 +774,17 @@ def _norm_operand(client: ComputeClient, t: Optional[TensorHandle], shape, dtype
         return None, 0
     if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
         raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: expected {tuple(shape)} {dtype.name}, got {tuple(t.shape)} {t.dtype.name}")
+    if len(shape) == 2 and t.strides[1] == 1 and t.strides[0] >= shape[1] > 0:
+        return t, t.strides[0]
     t, (_, _, stride) = _consumable(client, t, _norm_rows, what)
     return t, stride
 
 
 def _flat(t: Optional[TensorHandle], shape, dtypes, what: str):
     """A contiguous operand of this shape (axes of one aside) and one of these dtypes."""
-    if t is not None and ([d for d in t.shape if d != 1] != [d for d in shape if d != 1] or t.dtype not in dtypes or not t.is_contiguous()):
+    if t is None or (t.shape == shape and t.strides == (1,) and t.dtype in dtypes):
+        return t
+    if ([d for d in t.shape if d != 1] != [d for d in shape if d != 1] or t.dtype not in dtypes or not t.is_contiguous()):
         raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: expected contiguous {tuple(shape)} {'/'.join(d.name for d in dtypes)}, got {tuple(t.shape)} {t.dtype.name}")
     return t
 
@@ -838,8 +834,8 @@ def rms_norm(client: ComputeClient, input: TensorHandle, weight: Optional[Tensor
                          dtype=int(input.dtype), dtype_weight=int(weight.dtype) if weight is not None else N.DTYPE_F32, dtype_out=int(output.dtype),
                          scale_block=block)
     client._s.check(client.lib.mi355_rms_norm(
-        client.ctx, client.on(x, res, weight, residual_out, output, scales, rstd), C.byref(desc), C.c_void_p(x.device_ptr()), _ptr(res), _ptr(weight),
-        _ptr(residual_out), C.c_void_p(output.device_ptr()), _ptr(scales), _ptr(rstd)))
+        client.ctx, client.on(x, res, weight, residual_out, output, scales, rstd), C.byref(desc), x.device_ptr(), _ptr(res), _ptr(weight),
+        _ptr(residual_out), output.device_ptr(), _ptr(scales), _ptr(rstd)))
 
 
 def rms_norm_backward(client: ComputeClient, grad_output: TensorHandle, hidden: TensorHandle, weight: Optional[TensorHandle], rstd: TensorHandle,
@@ -876,8 +872,8 @@ def rms_norm_backward(client: ComputeClient, grad_output: TensorHandle, hidden: 
         if need.value:
             ws = client.empty(need.value)
     client._s.check(client.lib.mi355_rms_norm_grad(
-        client.ctx, client.on(g, h, weight, rstd, s, grad_input, grad_weight, ws), C.byref(desc), C.c_void_p(g.device_ptr()), C.c_void_p(h.device_ptr()),
-        _ptr(weight), C.c_void_p(rstd.device_ptr()), _ptr(s), C.c_void_p(grad_input.device_ptr()), _ptr(grad_weight), _ptr(ws), need.value))
+        client.ctx, client.on(g, h, weight, rstd, s, grad_input, grad_weight, ws), C.byref(desc), g.device_ptr(), h.device_ptr(),
+        _ptr(weight), rstd.device_ptr(), _ptr(s), grad_input.device_ptr(), _ptr(grad_weight), _ptr(ws), need.value))
 
 
 class TensorList:
@@ -888,10 +884,11 @@ class TensorList:
         self.tensors = list(tensors)
         self.memories = list({id(t.handle.memory): t.handle for t in self.tensors}.values())    # one handle per allocation, for stream order
         self.spans = (N.TensorSpan * max(len(self.tensors), 1))()
+        self.kinds = [(tuple(t.shape), t.dtype, t.is_contiguous()) for t in self.tensors]
         for i, t in enumerate(self.tensors):
             if t.dtype not in (ElemType.F32, ElemType.BF16, ElemType.F16):
                 raise ServerError(N.E_UNSUPPORTED, f"TensorList: tensor {i} must be f32, bf16 or f16")
-            if t.is_contiguous():
+            if self.kinds[i][2]:
                 self.spans[i] = (t.device_ptr(), 1, t.num_elems(), t.num_elems(), int(t.dtype), 0)
             else:
                 rows, cols, stride = _norm_rows(t, f"TensorList: tensor {i}")
@@ -918,7 +915,7 @@ def global_norm(client: ComputeClient, tensors, output: TensorHandle) -> None:
     _flat(output, (1,), (ElemType.F32,), "global_norm: output")
     ws = _norm_workspace(client)
     client._s.check(client.lib.mi355_global_norm(client.ctx, client.on(*tensors.memories, output, ws), tensors.spans, len(tensors),
-                                                 C.c_void_p(output.device_ptr()), C.c_void_p(ws.device_ptr()), ws.size))
+                                                 output.device_ptr(), ws.device_ptr(), ws.size))
 
 
 def clip_by_global_norm(client: ComputeClient, tensors, max_norm: float, *, outputs=None, total_norm: Optional[TensorHandle] = None) -> None:
@@ -938,18 +935,16 @@ def clip_by_global_norm(client: ComputeClient, tensors, max_norm: float, *, outp
     ws = _norm_workspace(client)
     handles = tensors.memories if outputs is tensors else tensors.memories + outputs.memories
     client._s.check(client.lib.mi355_clip_by_global_norm(client.ctx, client.on(*handles, total_norm, ws), ins, outs, len(tensors), max_norm,
-                                                         _ptr(total_norm), C.c_void_p(ws.device_ptr()), ws.size))
+                                                         _ptr(total_norm), ws.device_ptr(), ws.size))
 
 
 def _span_pairs(tensors: TensorList, outputs: TensorList):
     """The spans of both sides, walked the same way: where one of a pair is contiguous and the other has padded rows, both go by rows."""
-    alike = True
-    for a, b in zip(tensors.tensors, outputs.tensors):
-        if tuple(a.shape) != tuple(b.shape) or a.dtype != b.dtype:
-            raise ServerError(N.E_INVALID_ARGUMENT, f"clip_by_global_norm: output {tuple(b.shape)} {b.dtype.name} for {tuple(a.shape)} {a.dtype.name}")
-        alike = alike and a.is_contiguous() == b.is_contiguous()
-    if alike:
+    if tensors.kinds == outputs.kinds:
         return tensors.spans, outputs.spans
+    for a, b in zip(tensors.kinds, outputs.kinds):
+        if a[:2] != b[:2]:
+            raise ServerError(N.E_INVALID_ARGUMENT, f"clip_by_global_norm: output {b[0]} {b[1].name} for {a[0]} {a[1].name}")
     sides = []
     for side in (tensors, outputs):
         spans = (N.TensorSpan * max(len(side), 1))()

@@ -3,6 +3,7 @@ classifier (crates/cubecl-std/src/tensor/matrix_batch_layout.rs:21-79)."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -72,7 +73,7 @@ class TensorHandle:
         return len(self.shape)
 
     def num_elems(self) -> int:
-        return int(np.prod(self.shape)) if self.shape else 1
+        return math.prod(self.shape)
 
     def can_mut(self) -> bool:
         return True

@@ -481,8 +481,8 @@ int32_t mi355_gemm_scaled_select(mi355_ctx *ctx, const mi355_gemm_scaled_desc *d
  * Outputs must not overlap operands or each other (residual == C above excepted); an overlap that can be told from the descriptors is refused.
  * NaN and infinities follow the formula; an activation of -inf is its limit (0 for relu, gelu and silu).
  * The exponentials are v_exp_f32 (relative error below 2^-22 for |z| < 1), erf is Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7).
- * Kernels that cannot run their epilogue in place write the f32 product to library-owned per-stream scratch first (batch x M x N x 4 bytes):
- * inside a capture window such a call needs one earlier call of the same size on that stream. */
+ * Every kernel that mi355_gemm may take runs the epilogue on its accumulators, or in the fold of its K slices: scratch, capture windows and
+ * the choice of kernel are mi355_gemm's (the persistent 256x256 forms are replaced by the same tile, one a workgroup). */
 enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_GELU = 2 /* z * Phi(z) */, MI355_ACT_GELU_TANH = 3 /* its tanh form */, MI355_ACT_SILU = 4 };
 typedef struct {
     const void *bias, *residual;
@@ -496,9 +496,6 @@ typedef struct {
 } mi355_gemm_epilogue;
 int32_t mi355_gemm_fused(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc, const mi355_gemm_epilogue *epilogue,
                          const void *a, const void *b, void *c);
-/* 1 in *out_fused: mi355_gemm_fused runs this descriptor's epilogue inside the product's kernel (or its split-K fold); 0: as a pass over the f32
- * product in scratch.  Host-side only, operands taken as 16-byte aligned. */
-int32_t mi355_gemm_fused_plan(const mi355_gemm_desc *desc, int32_t *out_fused);
 
 /* The epilogue's gradient: grad_pre = grad_out * act'(pre), grad_bias[n] = sum over the rows of that product before its rounding.  pre and
  * grad_pre have grad_out's type (F32, BF16, F16); pre may be NULL for MI355_ACT_NONE, grad_bias may be NULL, and so may grad_pre where only

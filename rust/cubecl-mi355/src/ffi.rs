@@ -345,7 +345,6 @@ unsafe extern "C" {
     // a linear layer's epilogue, norms over rows and over tensor lists, and their gradients
     pub fn mi355_gemm_fused(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_gemm_desc, epilogue: *const mi355_gemm_epilogue,
                             a: *const c_void, b: *const c_void, c: *mut c_void) -> i32;
-    pub fn mi355_gemm_fused_plan(desc: *const mi355_gemm_desc, out_fused: *mut i32) -> i32;
     pub fn mi355_gemm_fused_grad_workspace_bytes(desc: *const mi355_gemm_fused_grad_desc, out_bytes: *mut u64) -> i32;
     pub fn mi355_gemm_fused_grad(ctx: *mut mi355_ctx, stream: mi355_stream, desc: *const mi355_gemm_fused_grad_desc, grad_out: *const c_void,
                                  pre: *const c_void, grad_pre: *mut c_void, grad_bias: *mut c_void, workspace: *mut c_void,

@@ -14,7 +14,6 @@ namespace mi355 {
 void launch_rms_norm(hipStream_t, int32_t, int, const norm_args &) { ++log_.norm; }
 void launch_rms_norm_grad(hipStream_t, int32_t, const norm_grad_args &) { ++log_.norm_grad; }
 void launch_fold_columns(hipStream_t, const float *, int64_t, int64_t, int64_t, void *, int32_t) { ++log_.fold; }
-void launch_epilogue(hipStream_t, const float *, const mi355_gemm_epilogue &, void *, int64_t, int64_t, int64_t, int32_t, int64_t, int64_t) { ++log_.epilogue; }
 void launch_fused_grad(hipStream_t, int32_t, int32_t, const fused_grad_args &) { ++log_.fused_grad; }
 void launch_square_sums(hipStream_t, const flat_table &t, uint32_t grid, double *) { ++log_.sums; log_.chunks += t.chunks; log_.partials += grid; }
 void launch_square_sums(hipStream_t, const rows_table &t, uint32_t grid, double *) { ++log_.sums; log_.chunks += t.chunks; log_.partials += grid; }

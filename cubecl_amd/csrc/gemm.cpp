@@ -761,10 +761,30 @@ int32_t run_tail_split(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, 
 
 namespace {
 
+// Operands that would be copied before a matrix-core kernel can stage them, with an epilogue: gemm_edge.hip takes them as they lie, while the
+// product is small enough for its smaller tiles.  us, copies and product / edge: f32, any layout: 333 x 517 x 1001 42 / 19, 2000 x 2000 x 501 63 / 49,
+// 8001 x 1001 x 333 94 / 66, but 2001 x 2003 x 2005 (16 GFLOP) 179 / 251.  16-bit, both operands k-contiguous: 333 x 517 x 1001 23 / 14, 4001 x 4003 x
+// 1001 (32 GFLOP) 68 / 64, 4001 x 4003 x 4005 147 / 196; otherwise (pieces turned on their way into LDS) 8001 x 1001 x 333 50 / 26, 2001 x 2003 x
+// 2005 58 / 122.
+// f32 operands that the 128 x 128 kernel would take, too few such tiles for the chip and no long K to slice: 512^3 25 / 16, 1024 x 1024 x 512 40 / 20,
+// 2048 x 1024 x 512 41 / 28, 512 x 512 x 2048 29 / 22; not 1024^3 31 / 33 (K in slices there too), nor 2048 x 2048 x 256 27 / 31 (256 tiles).
+bool edge_wins(const mi355_gemm_desc &d, const void *a, const void *b, const void *c)
+{
+    const int32_t algo = select_auto(d, a, b, c);
+    const double flops = 2.0 * (double)d.m * (double)d.n * (double)d.k * (double)d.batch;
+    if (algo == MI355_GEMM_ALGO_F32_MFMA) return tiles_of(d, 128, 128) <= rule::CUS / 2 && (flops <= 1.1e9 || d.k <= 512);
+    if (algo != MI355_GEMM_ALGO_GENERIC) return false;
+    return flops <= (d.dtype_ab != MI355_DTYPE_F32 && !d.trans_a && d.trans_b ? 40e9 : 8e9);
+}
+
 // mi355_gemm of a validated descriptor, with the epilogue `ep` where one is given
 int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     mi355_gemm_desc d = desc;
+    if (ep && gemm_edge_supports(d) && (d.algo == MI355_GEMM_ALGO_EDGE || (d.algo == MI355_GEMM_ALGO_AUTO && edge_wins(d, a, b, c))))
+        return launch_gemm_edge(ctx, s, d, a, b, c, *ep);
+    if (d.algo == MI355_GEMM_ALGO_EDGE)
+        return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the edge kernel belongs to mi355_gemm_fused and takes f32, bf16 and f16 operands with k > 0");
     int32_t algo = d.algo == MI355_GEMM_ALGO_AUTO ? select_auto(d, a, b, c) : d.algo;
     if (d.algo == MI355_GEMM_ALGO_AUTO && algo == MI355_GEMM_ALGO_GENERIC) {
         mi355_gemm_desc nd;
@@ -789,6 +809,12 @@ int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, con
             }
         }
     }
+    // 8-bit operands, at most two 128 x 128 tiles a CU: two co-resident workgroups hide each other's epilogue where the square tile waits for its
+    // own (us, square / 128: 1777 x 4096 x 4096 with silu and residual 55.6 / 45.1, without 48.3 / 40.7, 2048 x 4096 x 4096 56.8 / 47.4; three tiles a
+    // CU the other way, 2560 x 4096 x 4096 57.3 / 79.6)
+    if (ep && d.algo == MI355_GEMM_ALGO_AUTO && algo == MI355_GEMM_ALGO_LP_256W4 && is_fp8(d.dtype_ab) && tiles_of(d, 128, 128) <= 2 * rule::CUS &&
+        gemm_lp128_supports(d, a, b, c))
+        algo = MI355_GEMM_ALGO_LP_128;
     // the persistent kernels carry no epilogue: the same tile, one tile a workgroup
     if (ep && (algo == MI355_GEMM_ALGO_LP_256P || algo == MI355_GEMM_ALGO_LP_256Q || algo == MI355_GEMM_ALGO_LP_256QM))
         algo = gemm_lp256m16_supports(d, a, b, c) ? MI355_GEMM_ALGO_LP_256M16 : MI355_GEMM_ALGO_LP_256W4;

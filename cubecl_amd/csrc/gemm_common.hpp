@@ -175,6 +175,9 @@ void launch_splitk_fold(hipStream_t s, const float *slabs, uint32_t splits, int6
 // D = product + C, one rounding (gemm_add.hip)
 void launch_add_c(hipStream_t s, const float *prod, const void *c_in, void *d_out, int64_t batch, int64_t m, int64_t n,
                   int32_t dtype_c, int64_t ldc, int64_t stride_c);
+// operands as they lie, whatever their layout and alignment (gemm_edge.hip); with an epilogue only
+bool gemm_edge_supports(const mi355_gemm_desc &d);
+int32_t launch_gemm_edge(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args &ep);
 bool gemm_f32_mfma_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 bool gemm_lp128_supports(const mi355_gemm_desc &d, const void *a, const void *b, const void *c);
 

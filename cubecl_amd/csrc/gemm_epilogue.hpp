@@ -6,8 +6,8 @@
 //   finish_one    one output, for kernels that store by element (few rows, few columns, edges of everything)
 //   tile_finish   a wave's block of 32 rows that has been staged through LDS in f32: eight columns a lane, so the bias and the column scales
 //                 stay in registers over all rows, and everything leaves in whole 16-byte pieces.  AHEAD: the residual's pieces of a block are
-//                 in flight while its accumulators are staged (one workgroup a CU: nothing else hides their latency); without it a piece is
-//                 fetched when it is needed (several workgroups a CU, and half the registers)
+//                 in flight while the block before it is worked on (one workgroup a CU: nothing else hides their latency); without it a piece
+//                 is fetched when it is needed (several workgroups a CU, and a third of the registers)
 #pragma once
 
 #include <type_traits>
@@ -69,8 +69,9 @@ struct tile_finish {
     int64_t b, row, col, m, ldc, stride_c;
     char *c;
     int valid;
-    float bias[8], cs[8], rs[AHEAD ? PIECES : 1];
-    vec8<DT_C> res[AHEAD ? PIECES : 1];
+    float bias[8], cs[8];
+    static constexpr bool BUFFERED = AHEAD && DT_C != MI355_DTYPE_F32;      // a second set of pieces (f32: the registers end)
+    struct pieces { float rs[AHEAD ? PIECES : 1]; vec8<DT_C> res[AHEAD ? PIECES : 1]; } now, next;
 
     // the lane's first row and column of the wave's block; `live` false: a lane beyond the block's columns
     __device__ __forceinline__ tile_finish(const epilogue_args &e, const gemm_args &g, int64_t batch, int64_t row_, int64_t col_, bool live)
@@ -89,14 +90,14 @@ struct tile_finish {
     {
         if constexpr (AHEAD) {
 #pragma unroll
-            for (int it = 0; it < PIECES; ++it) fetch_piece(it, row + at + it * RPI);
+            for (int it = 0; it < PIECES; ++it) fetch_piece(BUFFERED ? next : now, it, row + at + it * RPI);
         }
     }
-    __device__ __forceinline__ void fetch_piece(int slot, int64_t r)
+    __device__ __forceinline__ void fetch_piece(pieces &p, int slot, int64_t r)
     {
         const bool in = r < m && valid > 0;
-        rs[slot] = ep.p.row_scale && in ? ep.p.row_scale[b * ep.p.stride_row_scale + r * ep.p.inc_row_scale] : 1.0f;
-        if (ep.p.residual && in) res[slot] = load8<DT_C>(ep.p.residual, b * ep.p.stride_residual + r * ep.p.ld_residual + col, valid);
+        p.rs[slot] = ep.p.row_scale && in ? ep.p.row_scale[b * ep.p.stride_row_scale + r * ep.p.inc_row_scale] : 1.0f;
+        if (ep.p.residual && in) p.res[slot] = load8<DT_C>(ep.p.residual, b * ep.p.stride_residual + r * ep.p.ld_residual + col, valid);
     }
     template <int KIND>
     __device__ __forceinline__ void piece(const char *rd, int64_t r, int slot)
@@ -105,28 +106,91 @@ struct tile_finish {
         const f32x4 lo = *reinterpret_cast<const f32x4 *>(rd), hi = *reinterpret_cast<const f32x4 *>(rd + 16);
         float z[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) * (rs[slot] * cs[e]) + bias[e];
+        for (int e = 0; e < 8; ++e) z[e] = e < 4 ? lo[e & 3] : hi[e & 3];
+        if (ep.p.row_scale) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] *= now.rs[slot];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = z[e] * cs[e] + bias[e];
         if (ep.p.pre) store8<DT_C, true>(ep.p.pre, b * ep.p.stride_pre + r * ep.p.ld_pre + col, valid, z);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             z[e] = KIND == ACT_SIGMOID ? act_sigmoid(z[e], ep.a, ep.b) : KIND == ACT_ERF ? act_erf(z[e]) : act_linear(z[e], ep.floor);
-            if (ep.p.residual) z[e] += get(res[slot], e);
+            if (ep.p.residual) z[e] += get(now.res[slot], e);
         }
         store8<DT_C, true>(c, b * stride_c + r * ldc + col, valid, z);
     }
     template <int KIND>
     __device__ __forceinline__ void rows(const char *rd, int pitch, int at)
     {
-        if constexpr (AHEAD) {
-#pragma unroll
-            for (int it = 0; it < PIECES; ++it) piece<KIND>(rd + it * RPI * pitch, row + at + it * RPI, it);
-        } else {
 #pragma unroll 1
-            for (int it = 0; it < PIECES; ++it) {
-                fetch_piece(0, row + at + it * RPI);
-                piece<KIND>(rd + it * RPI * pitch, row + at + it * RPI, 0);
-            }
+        for (int it = 0; it < PIECES; ++it) {
+            fetch_piece(now, 0, row + at + it * RPI);
+            piece<KIND>(rd + it * RPI * pitch, row + at + it * RPI, 0);
         }
+    }
+    // AHEAD: GROUP pieces of the block through each step together, so that one piece's LDS reads and exponentials hide another's; INSIDE: every
+    // row is one.  (Eight at once do not fit the registers beside 256 accumulators; 1 / 4: up projection of 4096 x 8192 x 2048, gelu and kept
+    // pre-activation, 138.8 / 133.8 us, 8-bit 1777 x 4096 x 4096 58.8 / 55.2.)
+    static constexpr int GROUP = DT_C == MI355_DTYPE_F32 ? 1 : PIECES < 4 ? PIECES : 4;
+    template <int KIND>
+    static __device__ __forceinline__ void act_all(float (&z)[GROUP][8], float a, float b, float floor)
+    {
+#pragma unroll
+        for (int it = 0; it < GROUP; ++it)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[it][e] = KIND == ACT_SIGMOID ? act_sigmoid(z[it][e], a, b) : KIND == ACT_ERF ? act_erf(z[it][e]) : act_linear(z[it][e], floor);
+    }
+    template <bool INSIDE>
+    __device__ __forceinline__ void store_all(void *p, int64_t at_, int64_t ld, int64_t r0, const float (&z)[GROUP][8])
+    {
+#pragma unroll
+        for (int it = 0; it < GROUP; ++it)
+            if (INSIDE || r0 + it * RPI < m) store8<DT_C, true>(p, at_ + it * RPI * ld, INSIDE ? 8 : valid, z[it]);
+    }
+    template <bool INSIDE>
+    __device__ __forceinline__ void together(const char *rd, int pitch, int at, const float *rs, const vec8<DT_C> *res)
+    {
+        float z[GROUP][8];
+#pragma unroll
+        for (int it = 0; it < GROUP; ++it) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(rd + it * RPI * pitch), hi = *reinterpret_cast<const f32x4 *>(rd + it * RPI * pitch + 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[it][e] = e < 4 ? lo[e & 3] : hi[e & 3];
+        }
+        if (valid > 0) {
+            const int64_t r0 = row + at;
+            if (ep.p.row_scale) {
+#pragma unroll
+                for (int it = 0; it < GROUP; ++it)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[it][e] *= rs[it];
+            }
+            if (ep.p.col_scale) {
+#pragma unroll
+                for (int it = 0; it < GROUP; ++it)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[it][e] = z[it][e] * cs[e] + bias[e];
+            } else if (ep.p.bias) {
+#pragma unroll
+                for (int it = 0; it < GROUP; ++it)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[it][e] += bias[e];
+            }
+            if (ep.p.pre) store_all<INSIDE>(ep.p.pre, b * ep.p.stride_pre + r0 * ep.p.ld_pre + col, ep.p.ld_pre, r0, z);
+            if (ep.kind == ACT_SIGMOID) act_all<ACT_SIGMOID>(z, ep.a, ep.b, 0.0f);
+            else if (ep.kind == ACT_ERF) act_all<ACT_ERF>(z, 0.0f, 0.0f, 0.0f);
+            else if (ep.floor == 0.0f) act_all<ACT_LINEAR>(z, 0.0f, 0.0f, 0.0f);
+            if (ep.p.residual) {
+#pragma unroll
+                for (int it = 0; it < GROUP; ++it)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[it][e] += get(res[it], e);
+            }
+            store_all<INSIDE>(c, b * stride_c + r0 * ldc + col, ldc, r0, z);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
     // All NB blocks: stage(block, as a constant) puts a block's accumulators into LDS, rows `pitch` bytes apart; `rd`: the lane's eight columns of
     // its first row there.  From three blocks up the loop is a loop -- the accumulators are named by a branch over the block's number, kept apart
@@ -139,9 +203,13 @@ struct tile_finish {
             one<0>(stage, rd, pitch);
             if constexpr (NB == 2) one<1>(stage, rd, pitch);
         } else {
+            if constexpr (BUFFERED) fetch(0);
 #pragma unroll 1
             for (int i = 0; i < NB; ++i) {
-                fetch(i * 32);
+                if constexpr (BUFFERED) {
+                    now = next;
+                    if (i + 1 < NB) fetch((i + 1) * 32);
+                } else fetch(i * 32);
                 stage_one(std::make_integer_sequence<int, NB>{}, i, stage);
                 finish_block(rd, pitch, i);
             }
@@ -151,6 +219,7 @@ struct tile_finish {
     __device__ __forceinline__ void one(STAGE &stage, const char *rd, int pitch)
     {
         fetch(I * 32);
+        if constexpr (BUFFERED) now = next;
         stage(std::integral_constant<int, I>{});
         finish_block(rd, pitch, I);
     }
@@ -175,7 +244,14 @@ struct tile_finish {
     // the block's rows, staged `pitch` bytes apart; `rd`: the lane's eight columns of its first row
     __device__ __forceinline__ void block(const char *rd, int pitch, int at)
     {
-        if (ep.kind == ACT_SIGMOID) rows<ACT_SIGMOID>(rd, pitch, at);
+        if constexpr (AHEAD) {
+            const bool inside = __all((valid == 8 || valid == 0) && row + at + (PIECES - 1) * RPI < m);
+#pragma unroll
+            for (int g = 0; g < PIECES; g += GROUP) {
+                if (inside) together<true>(rd + g * RPI * pitch, pitch, at + g * RPI, now.rs + g, now.res + g);
+                else together<false>(rd + g * RPI * pitch, pitch, at + g * RPI, now.rs + g, now.res + g);
+            }
+        } else if (ep.kind == ACT_SIGMOID) rows<ACT_SIGMOID>(rd, pitch, at);
         else if (ep.kind == ACT_ERF) rows<ACT_ERF>(rd, pitch, at);
         else rows<ACT_LINEAR>(rd, pitch, at);
     }

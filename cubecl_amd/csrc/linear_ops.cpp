@@ -42,7 +42,7 @@ bool float_type(int32_t t) { return t == MI355_DTYPE_F32 || t == MI355_DTYPE_BF1
 int64_t slab_rows(const mi355_gemm_fused_grad_desc &d)
 {
     const int64_t wide = (d.n + 511) / 512 * d.batch;
-    const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>({256, (d.m + 15) / 16, (4096 + wide - 1) / wide}));
+    const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>({256, (d.m + 3) / 4, (4096 + wide - 1) / wide}));
     return (d.m + slabs - 1) / slabs;
 }
 int64_t slab_count(const mi355_gemm_fused_grad_desc &d)

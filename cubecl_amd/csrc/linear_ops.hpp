@@ -22,7 +22,7 @@ struct norm_grad_args {
     const void *grad_out, *hidden, *weight, *grad_hidden;
     const float *rstd;
     void *grad_in;
-    float *partial;           // [workgroups x rows a workgroup holds at once][cols], NULL: no weight gradient
+    float *partial;           // [workgroups][cols], NULL: no weight gradient
     int64_t rows, cols, ld_out, ld_hidden, ld_in, ld_stream;
     float inv_cols;
     int32_t dtype_weight;
@@ -51,7 +51,7 @@ inline row_shape grad_shape_for(int64_t rows, int64_t cols)
     return sh.threads == 1024 && sh.pieces == 2 ? row_shape{512, 4} : sh;
 }
 
-// workgroups of the gradient: each walks rows / grid of them and leaves one partial row (four, T = 64) of the weight's gradient
+// workgroups of the gradient: each walks rows / grid of them and leaves one partial row of the weight's gradient
 constexpr int64_t GRAD_WGS = 512, LONG_SLABS = 64;
 inline int64_t norm_grad_wgs(int64_t rows, const row_shape &sh)
 {
@@ -61,7 +61,7 @@ inline int64_t norm_grad_partials(int64_t rows, int64_t cols)
 {
     const row_shape sh = grad_shape_for(rows, cols);
     if (sh.threads == 0) return std::min(rows, LONG_SLABS);
-    return norm_grad_wgs(rows, sh) * (sh.threads == 64 ? 4 : 1);
+    return norm_grad_wgs(rows, sh);
 }
 
 void launch_rms_norm(hipStream_t s, int32_t dtype, int mode, const norm_args &a);

@@ -338,11 +338,29 @@ rms_norm_grad_kernel(norm_grad_args a)
             store8<DT>(static_cast<char *>(a.grad_in) + row * a.ld_in * elem_size<DT>(), i, (int)min((int64_t)8, max((int64_t)0, a.cols - i)), d);
         }
     }
+    if constexpr (T == 64) {                                    // the four waves' rows meet before they leave
+        __shared__ float meet[3][CH * 8][64];
+        const int wave = threadIdx.x >> 6;
+        if (wave > 0) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) meet[wave - 1][c * 8 + e][t] = dw[c][e];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w4 = 0; w4 < 3; ++w4)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dw[c][e] += meet[w4][c * 8 + e][t];
+    }
     if (a.partial) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int64_t i = ((int64_t)c * T + t) * 8;
-            store8<MI355_DTYPE_F32>(a.partial + lane_row * a.cols, i, (int)min((int64_t)8, max((int64_t)0, a.cols - i)), dw[c]);
+            store8<MI355_DTYPE_F32>(a.partial + (int64_t)blockIdx.x * a.cols, i, (int)min((int64_t)8, max((int64_t)0, a.cols - i)), dw[c]);
         }
     }
 }

@@ -68,12 +68,6 @@ __device__ __forceinline__ float get(const vec8<DT> &r, int e)      // e a compi
     }
 }
 
-template <bool NT, class V>
-__device__ __forceinline__ void put(V *p, const V &v)
-{
-    if constexpr (NT) __builtin_nontemporal_store(v, p);
-    else *p = v;
-}
 // NT: past the caches, for outputs larger than they are
 template <int DT, bool NT = false>
 __device__ __forceinline__ void store8(void *p, int64_t i, int valid, const float (&f)[8])
@@ -83,8 +77,13 @@ __device__ __forceinline__ void store8(void *p, int64_t i, int valid, const floa
         if (valid >= 8) {
             const u32x4_e4 lo = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
             const u32x4_e4 hi = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
-            put<NT>(reinterpret_cast<u32x4_e4 *>(q), lo);
-            put<NT>(reinterpret_cast<u32x4_e4 *>(q + 4), hi);
+            if constexpr (NT) {
+                __builtin_nontemporal_store(lo, reinterpret_cast<u32x4_e4 *>(q));
+                __builtin_nontemporal_store(hi, reinterpret_cast<u32x4_e4 *>(q + 4));
+            } else {
+                *reinterpret_cast<u32x4_e4 *>(q) = lo;
+                *reinterpret_cast<u32x4_e4 *>(q + 4) = hi;
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -94,7 +93,8 @@ __device__ __forceinline__ void store8(void *p, int64_t i, int valid, const floa
         uint16_t *q = static_cast<uint16_t *>(p) + i;
         if (valid >= 8) {
             const u32x4_e2 v = {f32x2_to_lp<DT>(f[0], f[1]), f32x2_to_lp<DT>(f[2], f[3]), f32x2_to_lp<DT>(f[4], f[5]), f32x2_to_lp<DT>(f[6], f[7])};
-            put<NT>(reinterpret_cast<u32x4_e2 *>(q), v);
+            if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_e2 *>(q));
+            else *reinterpret_cast<u32x4_e2 *>(q) = v;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)

@@ -634,7 +634,7 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
         grad_lhs = grad_pre @ rhs^T                   grad_rhs = lhs^T @ grad_pre
 
     and the residual's gradient is grad_out itself.  Outputs that are not given are not computed; grad_pre (grad_out's shape and dtype, f32, bf16
-    or f16; may be grad_out or pre_activation itself) is needed for the products, which `matmul` takes from it as it is stored; grad_bias sums it before its rounding.
+    or f16; may be grad_out or pre_activation itself) is needed for the products, which take it as it is stored; grad_bias sums it before its rounding.
     `pre_activation` may be None for activation "none".  grad_bias: [n] or [batch.., n], f32 or grad_out's dtype.  An operand that matmul_fused
     broadcast over the batch gets the sum over the batch."""
     what = "matmul_fused_backward"
@@ -701,16 +701,16 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
     if grad_lhs is not None:
         lead = grad_lhs.num_elems() // (m * grad_lhs.shape[-1]) if grad_lhs.num_elems() else batch
         if lead == batch or grad_lhs.num_elems() == 0:
-            matmul(client, grad_pre, _swap_last(rhs), _with_batch_of(grad_lhs, grad_out))
+            matmul_fused(client, grad_pre, _swap_last(rhs), _with_batch_of(grad_lhs, grad_out))
         else:                                       # one lhs for all entries: their sum, in f32 until the last
             _sum_of_products(client, [(_entry(grad_pre, b), _swap_last(_entry(rhs, b))) for b in range(batch)], grad_lhs)
     if grad_rhs is not None:
         lead = grad_rhs.num_elems() // (n * grad_rhs.shape[-2]) if grad_rhs.num_elems() else batch
         left_lead = lhs.num_elems() // (m * lhs.shape[-1]) if lhs.num_elems() else batch
         if lead == batch or grad_rhs.num_elems() == 0:
-            matmul(client, _swap_last(lhs), grad_pre, _with_batch_of(grad_rhs, grad_out))
+            matmul_fused(client, _swap_last(lhs), grad_pre, _with_batch_of(grad_rhs, grad_out))
         elif left_lead == batch:                    # one rhs for all entries: their rows under each other are one product
-            matmul(client, _swap_last(_as_rows(client, lhs)), _as_rows(client, grad_pre), _entry(grad_rhs, 0))
+            matmul_fused(client, _swap_last(_as_rows(client, lhs)), _as_rows(client, grad_pre), _entry(grad_rhs, 0))
         else:
             _sum_of_products(client, [(_swap_last(_entry(lhs, b)), _entry(grad_pre, b)) for b in range(batch)], grad_rhs)
 

@@ -406,8 +406,10 @@ enum {
     MI355_GEMM_ALGO_LP_192X192 = 13, /* ... and on a 192 x 192 tile (each wave 96 x 96; NJ = NI = 3) */
     MI355_GEMM_ALGO_LP_256M16 = 14,  /* bf16/f16, [N][K] rhs: the 256 x 256 tile on v_mfma_f32_16x16x32 (eight MFMAs per A fragment: the
                                      order that issues at 16 cycles and holds a higher clock on random operands; gemm_lp256m16.hip) */
-    MI355_GEMM_ALGO_LP_256QM = 15    /* bf16/f16, [N][K] rhs, 16-bit C, full tiles: the persistent dripped-store kernel (_LP_256Q) on the 16x16x32
+    MI355_GEMM_ALGO_LP_256QM = 15,   /* bf16/f16, [N][K] rhs, 16-bit C, full tiles: the persistent dripped-store kernel (_LP_256Q) on the 16x16x32
                                      MFMA order of _LP_256M16; bit-identical to _LP_256M16 (ABI 9; gemm_lp256qm.hip, config C5) */
+    MI355_GEMM_ALGO_EDGE = 16        /* mi355_gemm_fused only: f32 / bf16 / f16 operands of any layout, size and alignment as they lie, no
+                                     re-layout (gemm_edge.hip); AUTO takes it there where the copies would cost more than its smaller tiles */
 };
 
 int32_t mi355_gemm(mi355_ctx *ctx, mi355_stream stream, const mi355_gemm_desc *desc,

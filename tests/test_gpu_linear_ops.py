@@ -194,12 +194,24 @@ def test_fused_on_every_kernel(client, m, n, k, dt, rhs):
 
 
 ALGOS = {"generic": N.GEMM_ALGO_GENERIC, "lp128": N.GEMM_ALGO_LP_128, "lp256w4": N.GEMM_ALGO_LP_256W4, "lp256x128": N.GEMM_ALGO_LP_256X128, "lp256x192": N.GEMM_ALGO_LP_256X192,
-         "lp192x192": N.GEMM_ALGO_LP_192X192, "lp256m16": N.GEMM_ALGO_LP_256M16, "lp256p": N.GEMM_ALGO_LP_256P, "lp256qm": N.GEMM_ALGO_LP_256QM}
+         "lp192x192": N.GEMM_ALGO_LP_192X192, "lp256m16": N.GEMM_ALGO_LP_256M16, "lp256p": N.GEMM_ALGO_LP_256P, "lp256qm": N.GEMM_ALGO_LP_256QM, "edge": N.GEMM_ALGO_EDGE}
 
 
 @pytest.mark.parametrize("algo", sorted(ALGOS))
 def test_fused_on_a_named_kernel(client, algo):
     run_fused(client, 512, 768, 512, BF16, BF16, "gelu_tanh", bias=F32, residual=True, pre=True, rhs="nk", algo=ALGOS[algo], seed=8)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 5, 2), (31, 33, 7), (64, 64, 64), (65, 129, 63), (70, 66, 65), (100, 200, 517), (257, 130, 1001), (2050, 2049, 99), (33, 40, 4001)])
+@pytest.mark.parametrize("dt", FLOATS, ids=lambda d: d.name)
+@pytest.mark.parametrize("layout", ["mk,kn", "mk,nk", "km,kn", "km,nk"])
+def test_fused_on_the_edge_kernel(client, m, n, k, dt, layout):
+    """Every layout at sizes and alignments that nothing else stages as they lie; long K in slices."""
+    lhs, rhs = layout.split(",")
+    run_fused(client, m, n, k, dt, dt, "gelu_tanh", bias=dt, residual=True, pre=True, lhs=lhs, rhs=rhs, seed=m + k, algo=N.GEMM_ALGO_EDGE)
+    if dt != F32:
+        run_fused(client, m, n, k, dt, F32, "none", lhs=lhs, rhs=rhs, seed=m, algo=N.GEMM_ALGO_EDGE)
+    run_fused(client, min(m, 80), min(n, 80), min(k, 80), dt, dt, "silu", bias=dt, scales="rc", batch=(3,), lhs=lhs, rhs=rhs, seed=n, algo=N.GEMM_ALGO_EDGE)
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 64, 128), (5, 40, 33), (16, 256, 256), (100, 96, 384), (257, 300, 512), (1030, 1040, 256)])

@@ -540,8 +540,8 @@ int32_t relayout_for_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &
         const int64_t nba = d.stride_a == 0 ? 1 : d.batch;
         void *q = nullptr;
         if (scratch_get(ctx, s, SCRATCH_RELAYOUT_A, (size_t)(nba * d.m * p.kpad * esz), &q) != MI355_OK) return MI355_E_UNSUPPORTED;
-        if (d.trans_a) {                                                       // [K][M] -> [M][kpad], pad columns zeroed first
-            if (p.kpad != d.k) (void)hipMemsetAsync(q, 0, (size_t)(nba * d.m * p.kpad * esz), s);
+        if (d.trans_a) {                                                       // [K][M] -> [M][kpad], zeros in the pad columns
+            if (p.kpad != d.k) launch_zero_columns(s, q, nba * d.m, d.k * esz, p.kpad * esz);
             launch_transpose(s, a, q, d.k, d.m, d.lda, p.kpad, nba, d.stride_a, d.m * p.kpad, esz);
         } else {
             launch_pad_copy(s, a, q, d.m, d.k, p.kpad, d.lda, p.kpad, nba, d.stride_a, d.m * p.kpad, esz);
@@ -553,7 +553,7 @@ int32_t relayout_for_mfma(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &
         void *q = nullptr;
         if (scratch_get(ctx, s, SCRATCH_RELAYOUT_B, (size_t)(nbb * d.n * p.kpad * esz), &q) != MI355_OK) return MI355_E_UNSUPPORTED;
         if (!d.trans_b) {                                                      // [K][N] -> [N][kpad]
-            if (p.kpad != d.k) (void)hipMemsetAsync(q, 0, (size_t)(nbb * d.n * p.kpad * esz), s);
+            if (p.kpad != d.k) launch_zero_columns(s, q, nbb * d.n, d.k * esz, p.kpad * esz);
             launch_transpose(s, b, q, d.k, d.n, d.ldb, p.kpad, nbb, d.stride_b, d.n * p.kpad, esz);
         } else {
             launch_pad_copy(s, b, q, d.n, d.k, p.kpad, d.ldb, p.kpad, nbb, d.stride_b, d.n * p.kpad, esz);

@@ -246,7 +246,7 @@ namespace mi355 {
 bool gemm_edge_supports(const mi355_gemm_desc &d)
 {
     if (d.dtype_ab != MI355_DTYPE_F32 && d.dtype_ab != MI355_DTYPE_BF16 && d.dtype_ab != MI355_DTYPE_F16) return false;
-    return d.k > 0 && d.batch <= 65535 && tiles_at(d, 64) * d.batch < (1ll << 31);
+    return d.k > 0 && d.batch <= 65535 && tiles_at(d, 64) * d.batch < (1ll << 24);      // (a launch holds fewer than 2^32 threads)
 }
 
 int32_t launch_gemm_edge(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d, const void *a, const void *b, void *c, const epilogue_args &ep)

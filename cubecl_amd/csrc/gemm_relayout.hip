@@ -93,6 +93,14 @@ pad_copy_kernel(const T *__restrict__ src, T *__restrict__ dst, int64_t rows, in
     }
 }
 
+// bytes [first, row_bytes) of every row (a kernel, not a memset: a memset node of a captured graph has given wrong results on later replays)
+__global__ void __launch_bounds__(256)
+zero_columns_kernel(uint8_t *__restrict__ dst, int64_t rows, int64_t first, int64_t row_bytes)
+{
+    const int64_t width = row_bytes - first;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * width; i += (int64_t)gridDim.x * 256) dst[i / width * row_bytes + first + i % width] = 0;
+}
+
 }  // namespace
 
 namespace mi355 {
@@ -114,6 +122,14 @@ void launch_pad_copy(hipStream_t s, const void *src, void *dst, int64_t rows, in
     else
         hipLaunchKernelGGL(pad_copy_kernel<uint32_t>, grid, dim3(256), 0, s, static_cast<const uint32_t *>(src),
                            static_cast<uint32_t *>(dst), rows, cols, cols_pad, ld_src, ld_dst, stride_src, stride_dst, vec_ok);
+}
+
+void launch_zero_columns(hipStream_t s, void *dst, int64_t rows, int64_t first_byte, int64_t row_bytes)
+{
+    const int64_t bytes = rows * (row_bytes - first_byte);
+    if (bytes <= 0) return;
+    hipLaunchKernelGGL(zero_columns_kernel, dim3((uint32_t)std::min<int64_t>((bytes + 255) / 256, 65536)), dim3(256), 0, s, static_cast<uint8_t *>(dst), rows, first_byte,
+                       row_bytes);
 }
 
 void launch_transpose(hipStream_t s, const void *src, void *dst, int64_t rows, int64_t cols, int64_t ld_src, int64_t ld_dst,

@@ -464,7 +464,10 @@ namespace mi355 {
 // `batch` sums of `count` partial rows each, [batch][count][cols] -> out [batch][cols]
 void launch_fold_columns(hipStream_t s, const float *partial, int64_t count, int64_t cols, int64_t batch, void *out, int32_t dtype)
 {
-    hipLaunchKernelGGL(fold_columns_kernel, dim3((uint32_t)((cols + 63) / 64), (uint32_t)batch), dim3(1024), 0, s, partial, count, cols, out, dtype);
+    const int64_t wide = (cols + 63) / 64, most = std::clamp<int64_t>((1 << 21) / wide, 1, 65535);      // (a launch holds fewer than 2^32 threads)
+    for (int64_t b = 0; b < batch; b += most)
+        hipLaunchKernelGGL(fold_columns_kernel, dim3((uint32_t)wide, (uint32_t)std::min(most, batch - b)), dim3(1024), 0, s, partial + b * count * cols, count, cols,
+                           static_cast<char *>(out) + b * cols * (int64_t)dtype_size(dtype), dtype);
 }
 
 }  // namespace mi355

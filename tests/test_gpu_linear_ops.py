@@ -837,6 +837,33 @@ def test_captured_steps(client):
             client.graph_destroy(g)
 
 
+@pytest.mark.parametrize("m,n,k,layout", [(2101, 2103, 1003, "mk,kn"), (2101, 2103, 1003, "km,kn"), (301, 203, 99, "km,nk"), (1024, 512, 8192, "mk,nk")])
+def test_captured_products_of_any_size(client, m, n, k, layout):
+    """Operands that are copied and zero-padded first, the edge kernel and K slices, captured and replayed with eager work of the same kind between."""
+    g = rng(m)
+    lhs, rhs = layout.split(",")
+    a, b, v = rand(g, m, k, dt=BF16), rand(g, k, n, dt=BF16, scale=k ** -0.5), rand(g, n, dt=BF16)
+    ta = up(client, a) if lhs == "mk" else up(client, a.t().contiguous()).permute((1, 0))
+    tb = up(client, b) if rhs == "kn" else up(client, b.t().contiguous()).permute((1, 0))
+    tv, out, other = up(client, v), empty(client, (m, n), BF16), empty(client, (m, n), BF16)
+    call = lambda o: ops.matmul_fused(client, ta, tb, o, bias=tv, activation="silu")
+    call(out)
+    z = a.double() @ b.double() + v.double()
+    y = act64("silu", z)[0]
+    close(down(client, out), y, rounded(y, act_tol("silu", z, 1e-5 * (a.double().abs() @ b.double().abs()) + 2.0 ** -22 * z.abs()), BF16))
+    want = raw_down(client, out)
+    graph = client.capture(lambda: call(out))
+    try:
+        for _ in range(3):
+            client._s.check(client.lib.mi355_memset(client.ctx, client.on(out), C.c_void_p(out.device_ptr()), 0xFF, m * n * 2))
+            client.replay(graph)
+            call(other)
+            client.sync()
+            assert torch.equal(raw_down(client, out), want) and torch.equal(raw_down(client, other), want)
+    finally:
+        client.graph_destroy(graph)
+
+
 def test_refusals_leave_the_output_alone(client):
     a, b = up(client, torch.ones(4, 8)), up(client, torch.ones(8, 8))
     c = up(client, torch.full((4, 8), 7.0))

@@ -29,7 +29,9 @@ struct norm_grad_args {
 };
 
 // Threads and pieces for rows of `cols` elements (0 threads: the looping kernels).  Few rows leave most of the chip idle, and then
-// the row's own latency is what is waited for: as many threads as hold it in one piece.
+// the row's own latency is what is waited for: as many threads as hold it in one piece.  bf16, us, 1024 threads / 256: 8 x 8192 3.7 / 5.1,
+// 256 x 4096 4.5 / 5.0, 512 x 8192 7.5 / 7.9, but 1024 x 4096 11.1 / 6.6, 1024 x 8192 13.6 / 11.6, 8192 x 4096 67 / 29 (a barrier's wait for sixteen
+// waves has no other workgroup on the CU to hide behind).  One wave / 256 threads for 4096 rows of 1024: 6.7 / 9.3.
 struct row_shape { int threads, pieces; };
 inline row_shape shape_for(int64_t rows, int64_t cols)
 {
@@ -44,14 +46,19 @@ inline row_shape shape_for(int64_t rows, int64_t cols)
     return {1024, 2};
 }
 
-// The gradient keeps the weight and its gradient in registers too: its longest rows take half the threads with twice the registers each.
+// The gradient keeps the weight and its gradient in registers too: rows above 4096 are held by 1024 threads in one piece (us, 1024 / 256
+// threads: 512 x 8192 13.7 / 17.8, 1024 x 8192 18.3 / 21.6, 4096 x 8192 45.2 / 48.5, but 2048 x 4096 18.9 / 18.1 and 8192 x 4096 51.5 / 42.8), the
+// longest by half the threads with twice the registers each (1024 x 2 pieces spills).
 inline row_shape grad_shape_for(int64_t rows, int64_t cols)
 {
+    if (cols > 4096 && cols <= 8192) return {1024, 1};
     const row_shape sh = shape_for(rows, cols);
     return sh.threads == 1024 && sh.pieces == 2 ? row_shape{512, 4} : sh;
 }
 
-// workgroups of the gradient: each walks rows / grid of them and leaves one partial row of the weight's gradient
+// workgroups of the gradient: each walks rows / grid of them and leaves one partial row of the weight's gradient.  Two (512 threads and up: one)
+// a CU; us, 512 / 256 workgroups: 2048 x 4096 18.1 / 20.7, 8192 x 4096 42.8 / 56.9, 512 x 8192 13.7 / 15.2; 1024 workgroups leave
+// twice the partial rows to fold: 2048 x 4096 19.9, 8192 x 4096 49.4, 512 x 8192 15.9.
 constexpr int64_t GRAD_WGS = 512, LONG_SLABS = 64;
 inline int64_t norm_grad_wgs(int64_t rows, const row_shape &sh)
 {

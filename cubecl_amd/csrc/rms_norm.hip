@@ -7,6 +7,8 @@
 // hidden + out bytes per element and nothing else; the weight comes out of L2.
 //   - T threads hold a row, CH pieces of eight consecutive elements each: piece c of thread t is elements (c T + t) 8 .. + 7, so a wave's
 //     16-byte accesses are one contiguous run.  T = 64: a wave by itself, four rows a workgroup, no barrier.
+//     bf16: 8192 x 4096 29 us (134 MB: 4.6 TB/s), 16384 x 4096 with the addition and an e4m3 output in blocks of 32 85 us (470 MB, 5.5 TB/s),
+//     8 x 4096 3.8 us, which is the latency of one load, one reduction and one store; the gradient of 8192 x 4096 43 us (201 MB, 4.7 TB/s, its fold included).
 //   - rows longer than 16384 elements (what 1024 threads hold in two pieces) are walked in a loop and read again, from L2.
 //   - 8-bit output: the scale needs the row's (block's) largest |y| first, which is in registers by then.  v_cvt_pk_fp8_f32 / _bf8_f32 round
 //     to nearest even; the scale keeps every quotient at or below MAX (1 + 2^-22), which rounds to MAX, so nothing saturates.

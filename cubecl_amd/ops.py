@@ -665,6 +665,14 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
         if t is not None and t.num_elems() // max(t.shape[-2] * t.shape[-1], 1) not in (1, batch) and t.num_elems():
             raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: {name} does not broadcast to batch {batch}")
 
+    # what one launch writes before another one reads (each launch checks its own operands)
+    late = [(t, *_extent(t)) for t, wanted in ((rhs, grad_lhs), (lhs, grad_rhs)) if wanted is not None]
+    outs = [(t, *_extent(t)) for t in (grad_pre, grad_bias, grad_lhs, grad_rhs) if t is not None] if late else []
+    for i, (o, first, end) in enumerate(outs):
+        for t, t_first, t_end in late + outs[:i]:
+            if first < t_end and t_first < end and _meshed(o, t, t_first - first):
+                raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: an output overlaps an operand or another output")
+
     def rows(t, name, writable=False):
         try:
             return t, _rows_of_matrix(t, batch, f"{what}: {name}")
@@ -713,6 +721,29 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
             matmul_fused(client, _swap_last(_as_rows(client, lhs)), _as_rows(client, grad_pre), _entry(grad_rhs, 0))
         else:
             _sum_of_products(client, [(_swap_last(_entry(lhs, b)), _entry(grad_pre, b)) for b in range(batch)], grad_rhs)
+
+
+def _extent(t: TensorHandle):
+    """(first byte, one past the last); empty for an empty tensor."""
+    first, last = t.device_ptr(), 0
+    for d, s in zip(t.shape, t.strides):
+        if d == 0:
+            return first, first
+        last += (d - 1) * s
+    return first, first + (last + 1) * t.dtype.size()
+
+
+def _meshed(a: TensorHandle, b: TensorHandle, distance: int) -> bool:
+    """Of two tensors whose extents meet, b `distance` bytes after a: do they share a byte?  False for column ranges of the same wider rows that
+    lie beside each other; other views that mesh without touching are taken as sharing."""
+    for t in (a, b):
+        if t.rank() < 2 or t.strides[-1] != 1 or any(t.strides[i] != t.strides[i + 1] * t.shape[i + 1] for i in range(t.rank() - 2)):
+            return True
+    ld = a.strides[-2] * a.dtype.size()
+    if ld == 0 or ld != b.strides[-2] * b.dtype.size():
+        return True
+    at = distance % ld
+    return at < a.shape[-1] * a.dtype.size() or at + b.shape[-1] * b.dtype.size() > ld
 
 
 def _with_batch_of(t: TensorHandle, model: TensorHandle) -> TensorHandle:

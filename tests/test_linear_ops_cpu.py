@@ -175,6 +175,26 @@ def test_fused_backward_refusals(client):
     assert client.lib.mi355_gemm_fused_grad_workspace_bytes(C.byref(desc), C.byref(need)) == N.E_INVALID_ARGUMENT
 
 
+def test_fused_backward_refuses_outputs_on_what_a_later_launch_reads(client):
+    """grad_lhs is complete before grad_rhs reads lhs, and grad_pre before either product reads the operands."""
+    m, n, k = 4, 6, 5
+    g, d = make(client, (m, n), BF16), make(client, (m, n), BF16)
+    a, b, da, db = make(client, (m, k), BF16), make(client, (k, n), BF16), make(client, (m, k), BF16), make(client, (k, n), BF16)
+    f = lambda pre, **kw: refused(ops.matmul_fused_backward, client, g, None, pre, match="overlaps", **{**dict(lhs=a, rhs=b, grad_lhs=da, grad_rhs=db), **kw})
+    f(d, grad_lhs=a)
+    f(d, grad_rhs=b)
+    f(d, grad_lhs=d, lhs=make(client, (m, n), BF16), rhs=make(client, (n, n), BF16), grad_rhs=None)
+    f(d, grad_rhs=make(client, (k, n), BF16, handle=da.handle))
+    f(d, grad_bias=make(client, (n,), BF16, handle=b.handle))
+    f(make(client, (m, n), BF16, handle=client.empty(256)), lhs=make(client, (m, k), BF16, (20, 1), d.handle), grad_lhs=make(client, (m, k), BF16, (20, 1), d.handle))
+    assert log(client)["fused_grad"] == 0
+    # column ranges of one wider matrix lie beside each other
+    wide = client.empty(m * 20 * 2)
+    left, right = TensorHandle.new(wide, (m, k), (20, 1), BF16), TensorHandle.new(wide.offset_start_by(2 * k), (m, k), (20, 1), BF16)
+    assert not ops._meshed(left, right, 2 * k) and not ops._meshed(right, left, -2 * k)
+    assert ops._meshed(left, right, 2 * k - 2) and ops._meshed(right, left, 2 - 2 * k)
+
+
 @pytest.mark.parametrize("m,n,batch", [(1, 1, 1), (4096, 8192, 1), (100000, 8, 1), (3, 100001, 1), (17, 40, 65535), (1 << 20, 512, 2)])
 def test_fused_backward_workspace_covers_its_slabs(client, m, n, batch):
     desc = N.GemmFusedGradDesc(m=m, n=n, batch=batch, ld_out=n, ld_pre=n, ld_grad=n, dtype=BF16, dtype_bias=F32)

@@ -137,7 +137,7 @@ void launch_epilogue(hipStream_t s, const float *prod, uint32_t slabs, int64_t s
                      int64_t n, int64_t ldc, int64_t stride_c)
 {
     const int64_t per_row = (n + 7) / 8, runs = m * per_row;
-    const dim3 grid((uint32_t)std::min<int64_t>((runs + 255) / 256, 1 << 20), (uint32_t)batch);
+    const dim3 grid((uint32_t)std::min<int64_t>((runs + 255) / 256, std::max<int64_t>(1, (1 << 20) / batch)), (uint32_t)batch);
     if (runs < (1ll << 31)) hipLaunchKernelGGL((epilogue_kernel<uint32_t>), grid, dim3(256), 0, s, prod, slabs, slab_stride, ep, c, (uint32_t)runs, (uint32_t)per_row, m, n, ldc, stride_c);
     else hipLaunchKernelGGL((epilogue_kernel<uint64_t>), grid, dim3(256), 0, s, prod, slabs, slab_stride, ep, c, (uint64_t)runs, (uint64_t)per_row, m, n, ldc, stride_c);
 }

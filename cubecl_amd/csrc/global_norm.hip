@@ -150,6 +150,7 @@ scale_kernel(TABLE tab, const double *__restrict__ partial, uint32_t count, floa
     const float coef = !(norm <= DBL_MAX) ? __uint_as_float(0x7FC00000u) : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.0f;
     for (uint32_t k = blockIdx.x; k < tab.chunks; k += gridDim.x) {
         const chunk_place p = place_of(tab, k);
+        if (coef == 1.0f && p.in == p.out) continue;              // in place and nothing to scale
         auto scale = [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
             each_run<DT>(p, [&](float (&x)[8], int64_t o, int valid) {

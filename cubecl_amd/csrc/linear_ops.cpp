@@ -53,7 +53,11 @@ int64_t slab_count(const mi355_gemm_fused_grad_desc &d)
     return (d.m + r - 1) / r;
 }
 
-bool grad_desc_sane(const mi355_gemm_fused_grad_desc &d) { return d.m >= 0 && d.n >= 0 && d.batch >= 0 && d.batch <= 65535; }
+// (a launch holds fewer than 2^32 threads: 8 columns each, 256 to a workgroup)
+bool grad_desc_sane(const mi355_gemm_fused_grad_desc &d)
+{
+    return d.m >= 0 && d.n >= 0 && d.batch >= 0 && d.batch <= 65535 && d.n <= (1ll << 31) / std::max<int64_t>(d.batch, 1);
+}
 uint64_t grad_bytes(const mi355_gemm_fused_grad_desc &d)
 {
     return d.m && d.n && d.batch ? (uint64_t)(d.batch * slab_count(d)) * (uint64_t)d.n * sizeof(float) : 0;
@@ -128,7 +132,7 @@ MI355_API int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, con
     MI355_REQUIRE_CTX(ctx);
     if (!desc) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: descriptor is NULL");
     const mi355_gemm_fused_grad_desc &d = *desc;
-    if (!grad_desc_sane(d)) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: a size is negative, or more than 65535 batch entries");
+    if (!grad_desc_sane(d)) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: a size is negative, or more than 65535 batch entries or 2^31 columns over the batch");
     if (d.dtype != MI355_DTYPE_F32 && d.dtype != MI355_DTYPE_BF16 && d.dtype != MI355_DTYPE_F16)
         return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm_fused_grad: unsupported dtype %d", d.dtype);
     if (d.activation < MI355_ACT_NONE || d.activation > MI355_ACT_SILU)

@@ -681,6 +681,20 @@ def test_clip_views(client):
     assert got[0] == line[0].double() and torch.equal(got[998:], line[998:].double())
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_clip_in_place_below_the_norm_changes_nothing(client, dt):
+    """Contiguous tensors and column ranges of wider ones, in place, with a norm below the limit: the same bits, and the norm all the same."""
+    g = rng(77)
+    a, b = rand(g, 5, 4099, dt=dt), rand(g, 130, 77, dt=dt)
+    ta, wide = up(client, a), up(client, b)
+    view = TensorHandle.new(wide.handle, (130, 40), (77, 1), dt)
+    before, norm = (raw_down(client, ta), raw_down(client, wide)), empty(client, (1,), F32)
+    ops.clip_by_global_norm(client, ops.TensorList([ta, view]), 1e6, total_norm=norm)
+    assert torch.equal(raw_down(client, ta), before[0]) and torch.equal(raw_down(client, wide), before[1])
+    want = float(torch.sqrt(a.double().pow(2).sum() + b[:, :40].double().pow(2).sum()))
+    assert abs(float(down(client, norm)[0]) - want) <= want * 2.0 ** -22
+
+
 def test_clip_special_values(client):
     """Squares beyond f32 on both sides; a NaN or an infinity anywhere makes every output NaN; zeros stay zeros."""
     out = empty(client, (1,), F32)

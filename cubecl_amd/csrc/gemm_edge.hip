@@ -263,10 +263,13 @@ int32_t launch_gemm_edge(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &d
     g.tiles_n = (uint32_t)((d.n + r - 1) / r);
     g.group_m = 8;
     g.split_k = 1;
+    // K slices while the tiles leave CUs idle, four steps a slice at least: a step's latency (1.5-2 us, its pieces' way from memory through registers)
+    // is what few tiles wait for.  us, eight steps a slice / four: f32 333 x 1001 x 517 20.0 / 18.2, 65 x 67 x 517 17.2 / 13.1, 30 x 2000 x 777 16.3 / 12.9,
+    // bf16 333 x 517 x 1001 20.5 / 14.5, 100 x 100 x 5001 22.6 / 18.4; f32 1001 x 517 x 333 18.1 / 18.5 (a fold for six steps less).
     int64_t splits = 1;
     float *slabs = nullptr;
-    if (tiles < cus && steps >= 16) {
-        splits = std::min<int64_t>({2 * cus / tiles, steps / 8, 32});
+    if (tiles < cus && steps >= 8) {
+        splits = std::min<int64_t>({2 * cus / tiles, steps / 4, 32});
         if (splits > 1) { const int64_t per = (steps + splits - 1) / splits; splits = (steps + per - 1) / per; }      // no empty slices
         if (splits > 1 && splitk_scratch(ctx, s, (size_t)(splits * d.batch * d.m * d.n) * sizeof(float), &slabs) != MI355_OK) splits = 1;
     }

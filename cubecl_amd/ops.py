@@ -616,13 +616,12 @@ def _as_rows(client: ComputeClient, t: TensorHandle) -> TensorHandle:
     if t.rank() == 2:
         return t
     rows, cols = math.prod(t.shape[:-1]), t.shape[-1]
-    acc, fits = t.strides[-2], True
-    for i in range(t.rank() - 3, -1, -1):
-        acc *= t.shape[i + 1]
-        fits = fits and (t.shape[i] == 1 or t.strides[i] == acc)
-    if not fits or (cols > 1 and t.strides[-1] != 1):
-        t = into_contiguous(client, t)
-    return TensorHandle.new(t.handle, (rows, cols), (max(t.strides[-2], cols), 1), t.dtype)
+    dims = [(d, s) for d, s in zip(t.shape[:-1], t.strides[:-1]) if d != 1]
+    ld = dims[-1][1] if dims else cols
+    # (rows that overlap -- an operand broadcast along them -- have no leading dimension)
+    if ld < cols or (cols > 1 and t.strides[-1] != 1) or any(s_out != s_in * d_in for (_, s_out), (d_in, s_in) in zip(dims[:-1], dims[1:])):
+        t, ld = into_contiguous(client, t), cols
+    return TensorHandle.new(t.handle, (rows, cols), (ld, 1), t.dtype)
 
 
 def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_activation: Optional[TensorHandle], grad_pre: Optional[TensorHandle], *,

@@ -764,8 +764,10 @@ def _entry(t: TensorHandle, b: int) -> TensorHandle:
 
 
 def _sum_of_products(client: ComputeClient, pairs, out: TensorHandle) -> None:
-    """out = sum of the products, accumulated in f32 and rounded once."""
+    """out = sum of the products, accumulated in f32 and rounded once; zeros where there are none (a batch of no entries)."""
     out = _entry(out, 0)
+    rows, cols = out.shape
+    pairs = pairs or [(TensorHandle.new_contiguous((rows, 0), client.empty(4), ElemType.F32), TensorHandle.new_contiguous((0, cols), client.empty(4), ElemType.F32))]
     total = TensorHandle.new_contiguous(out.shape, client.empty(out.num_elems() * 4), ElemType.F32)
     for i, (a, b) in enumerate(pairs):
         matmul(client, a, b, total, acc=total if i else None)

@@ -22,3 +22,14 @@ def test_backward_of_an_lhs_whose_rows_share_memory(client, dt, strides):
     ops.matmul_fused_backward(client, up(client, dy), None, dz, lhs=lhs, rhs=up(client, b), grad_rhs=dB)
     ref = a.reshape(-1, k).t() @ dy.double().reshape(-1, n)
     close(down(client, dB), ref, rounded(ref, 1e-5 * (a.reshape(-1, k).abs().t() @ dy.double().reshape(-1, n).abs()), dt))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=lambda d: d.name)
+def test_gradients_of_shared_operands_over_an_empty_batch(client, dt):
+    """Sums over no entries: zeros, for a weight, a left operand and a bias."""
+    one = lambda *s: up(client, torch.ones(s).to(torch.float32 if dt == F32 else torch.bfloat16))
+    for lhs_shape in ((4, 5), (0, 4, 5)):
+        da, db, bias = one(*lhs_shape), one(5, 6), one(6)
+        ops.matmul_fused_backward(client, empty(client, (0, 4, 6), dt), None, empty(client, (0, 4, 6), dt), grad_bias=bias,
+                                  lhs=one(*lhs_shape) if lhs_shape[0] else empty(client, lhs_shape, dt), rhs=one(5, 6), grad_lhs=da, grad_rhs=db)
+        assert all(bool((down(client, t) == 0).all()) for t in (da, db, bias))

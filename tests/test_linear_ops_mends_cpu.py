@@ -30,3 +30,15 @@ def test_a_batch_as_rows_is_the_same_elements(client, monkeypatch, shape, stride
     want = places(shape, make(client, shape).strides if copied else strides)
     assert np.array_equal(places(got.shape, got.strides), want)
     assert got.shape[0] <= 1 or got.strides[0] >= got.shape[1]
+
+
+# ---- a batch of no entries --------------------------------------------------------------------------------------------------------
+def test_gradients_of_shared_operands_over_an_empty_batch_are_written(client, monkeypatch):  # noqa: F811
+    """The sum over no entries is zeros: a product without a K axis, not whatever the memory held."""
+    done = []
+    monkeypatch.setattr(ops, "matmul", lambda c, a, b, out, acc=None: done.append((a.shape, b.shape, out.shape, acc)))
+    monkeypatch.setattr(ops, "copy_into", lambda c, a, out: done.append((a.shape, out.shape)))
+    g, d = make(client, (0, 4, 6)), make(client, (0, 4, 6))
+    a, b, da, db = make(client, (4, 5)), make(client, (5, 6)), make(client, (4, 5)), make(client, (5, 6))
+    ops.matmul_fused_backward(client, g, None, d, lhs=a, rhs=b, grad_lhs=da, grad_rhs=db)
+    assert done == [((4, 0), (0, 5), (4, 5), None), ((4, 5), (4, 5)), ((5, 0), (0, 6), (5, 6), None), ((5, 6), (5, 6))]

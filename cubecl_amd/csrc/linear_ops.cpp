@@ -53,7 +53,7 @@ int64_t slab_count(const mi355_gemm_fused_grad_desc &d)
     return (d.m + r - 1) / r;
 }
 
-// (a launch holds fewer than 2^32 threads: 8 columns each, 256 to a workgroup)
+// (a launch holds fewer than 2^32 threads: 8 columns each, 256 to a workgroup; the fold cuts its columns by itself)
 bool grad_desc_sane(const mi355_gemm_fused_grad_desc &d)
 {
     return d.m >= 0 && d.n >= 0 && d.batch >= 0 && d.batch <= 65535 && d.n <= (1ll << 31) / std::max<int64_t>(d.batch, 1);
@@ -239,7 +239,7 @@ MI355_API int32_t mi355_rms_norm(mi355_ctx *ctx, mi355_stream stream, const mi35
 
 MI355_API int32_t mi355_rms_norm_grad_workspace_bytes(const mi355_rms_norm_grad_desc *desc, uint64_t *out_bytes)
 {
-    if (!desc || !out_bytes || desc->rows < 0 || desc->cols < 0) return MI355_E_INVALID_ARGUMENT;
+    if (!desc || !out_bytes || desc->rows < 0 || desc->cols < 0 || desc->cols > GRAD_MAX_COLS) return MI355_E_INVALID_ARGUMENT;
     *out_bytes = desc->rows && desc->cols ? (uint64_t)norm_grad_partials(desc->rows, desc->cols) * (uint64_t)desc->cols * sizeof(float) : 0;
     return MI355_OK;
 }
@@ -251,7 +251,7 @@ MI355_API int32_t mi355_rms_norm_grad(mi355_ctx *ctx, mi355_stream stream, const
     MI355_REQUIRE_CTX(ctx);
     if (!desc) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: descriptor is NULL");
     const mi355_rms_norm_grad_desc &d = *desc;
-    if (d.rows < 0 || d.cols < 0) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: negative size");
+    if (d.rows < 0 || d.cols < 0 || d.cols > GRAD_MAX_COLS) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: a size is negative, or more than 2^31 columns");
     if (!float_type(d.dtype)) return fail(ctx, MI355_E_UNSUPPORTED, "mi355_rms_norm_grad: unsupported dtype %d", d.dtype);
     if ((d.dtype_weight != MI355_DTYPE_F32 && d.dtype_weight != d.dtype) ||
         (grad_weight && d.dtype_grad_weight != MI355_DTYPE_F32 && d.dtype_grad_weight != d.dtype))

@@ -59,20 +59,37 @@ inline row_shape grad_shape_for(int64_t rows, int64_t cols)
 // workgroups of the gradient: each walks rows / grid of them and leaves one partial row of the weight's gradient.  Two (512 threads and up: one)
 // a CU; us, 512 / 256 workgroups: 2048 x 4096 18.1 / 20.7, 8192 x 4096 42.8 / 56.9, 512 x 8192 13.7 / 15.2; 1024 workgroups leave
 // twice the partial rows to fold: 2048 x 4096 19.9, 8192 x 4096 49.4, 512 x 8192 15.9.
-constexpr int64_t GRAD_WGS = 512, LONG_SLABS = 64;
+constexpr int64_t GRAD_WGS = 512;
 inline int64_t norm_grad_wgs(int64_t rows, const row_shape &sh)
 {
     return std::min(sh.threads == 64 ? (rows + 3) / 4 : rows, sh.threads >= 512 ? GRAD_WGS / 2 : GRAD_WGS);
 }
+// ... and of the kernel for rows beyond the registers, eight columns a thread: slabs of rows, so that a launch keeps below 2^32 threads
+constexpr int64_t LONG_SLABS = 64, GRAD_MAX_COLS = 1ll << 31;
+inline int64_t norm_grad_slabs(int64_t rows, int64_t cols)
+{
+    return std::min(rows, std::clamp<int64_t>((1ll << 31) / ((cols + 2047) / 2048 * 256), 1, LONG_SLABS));
+}
 inline int64_t norm_grad_partials(int64_t rows, int64_t cols)
 {
     const row_shape sh = grad_shape_for(rows, cols);
-    if (sh.threads == 0) return std::min(rows, LONG_SLABS);
+    if (sh.threads == 0) return norm_grad_slabs(rows, cols);
     return norm_grad_wgs(rows, sh);
 }
 
 void launch_rms_norm(hipStream_t s, int32_t dtype, int mode, const norm_args &a);
 void launch_rms_norm_grad(hipStream_t s, int32_t dtype, const norm_grad_args &a);
+// Column sums take 1024 threads for 64 columns and a launch holds fewer than 2^32 threads: f(first column, workgroups wide, first batch entry,
+// batch entries) for each launch that `cols` columns of `batch` entries need.
+constexpr int64_t FOLD_COLS = 64, FOLD_WGS = 1 << 21;
+template <class F>
+void each_fold_launch(int64_t cols, int64_t batch, F f)
+{
+    for (int64_t c = 0; c < cols; c += FOLD_COLS * FOLD_WGS) {
+        const int64_t wide = (std::min(cols - c, FOLD_COLS * FOLD_WGS) + FOLD_COLS - 1) / FOLD_COLS, most = std::clamp<int64_t>(FOLD_WGS / wide, 1, 65535);
+        for (int64_t b = 0; b < batch; b += most) f(c, wide, b, std::min(most, batch - b));
+    }
+}
 // column sums of f32 partial rows, [batch][count][cols] -> out [batch][cols] in `dtype`; count 0: zeros
 void launch_fold_columns(hipStream_t s, const float *partial, int64_t count, int64_t cols, int64_t batch, void *out, int32_t dtype);
 

@@ -432,11 +432,11 @@ namespace {
 
 // out[c] = partial[0][c] + partial[1][c] + ...: 64 columns x 16 slices of the partial rows a workgroup, slices in order, then across them
 __global__ void __launch_bounds__(1024)
-fold_columns_kernel(const float *__restrict__ partial, int64_t count, int64_t cols, void *__restrict__ out, int32_t dtype)
+fold_columns_kernel(const float *__restrict__ partial, int64_t count, int64_t first_col, int64_t cols, void *__restrict__ out, int32_t dtype)
 {
     __shared__ float part[16][64];
     const int lane = threadIdx.x & 63, s = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = first_col + (int64_t)blockIdx.x * FOLD_COLS + lane;
     const float *p = partial + (int64_t)blockIdx.y * count * cols + c;
     const int64_t per = (count + 15) / 16, first = s * per, last = min(count, first + per);
     float acc = 0.0f;
@@ -466,10 +466,10 @@ namespace mi355 {
 // `batch` sums of `count` partial rows each, [batch][count][cols] -> out [batch][cols]
 void launch_fold_columns(hipStream_t s, const float *partial, int64_t count, int64_t cols, int64_t batch, void *out, int32_t dtype)
 {
-    const int64_t wide = (cols + 63) / 64, most = std::clamp<int64_t>((1 << 21) / wide, 1, 65535);      // (a launch holds fewer than 2^32 threads)
-    for (int64_t b = 0; b < batch; b += most)
-        hipLaunchKernelGGL(fold_columns_kernel, dim3((uint32_t)wide, (uint32_t)std::min(most, batch - b)), dim3(1024), 0, s, partial + b * count * cols, count, cols,
+    each_fold_launch(cols, batch, [&](int64_t c, int64_t wide, int64_t b, int64_t entries) {
+        hipLaunchKernelGGL(fold_columns_kernel, dim3((uint32_t)wide, (uint32_t)entries), dim3(1024), 0, s, partial + b * count * cols, count, c, cols,
                            static_cast<char *>(out) + b * cols * (int64_t)dtype_size(dtype), dtype);
+    });
 }
 
 }  // namespace mi355
@@ -497,7 +497,7 @@ void launch_norm_grad(hipStream_t s, const norm_grad_args &a)
     if (sh.threads == 0) {
         // (the weight's gradient first: grad_in may be one of the operands it reads)
         if (a.partial)
-            hipLaunchKernelGGL((rms_norm_grad_weight_long_kernel<DT>), dim3((uint32_t)((a.cols + 2047) / 2048), (uint32_t)std::min(a.rows, LONG_SLABS)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((rms_norm_grad_weight_long_kernel<DT>), dim3((uint32_t)((a.cols + 2047) / 2048), (uint32_t)norm_grad_slabs(a.rows, a.cols)), dim3(256), 0, s, a);
         hipLaunchKernelGGL((rms_norm_grad_long_kernel<DT>), dim3((uint32_t)std::min(a.rows, MAX_GRID)), dim3(1024), 0, s, a);
         return;
     }

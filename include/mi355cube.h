@@ -665,7 +665,7 @@ int32_t mi355_rms_norm(mi355_ctx *ctx, mi355_stream stream, const mi355_rms_norm
  *     grad_in = rstd * (w * g - x^ * mean(w * g * x^)) + grad_hidden        grad_weight = sum over rows of g * x^
  * grad_out (g), hidden, grad_in and grad_hidden (the gradient that reaches h by the residual stream; may be NULL, or grad_in itself) have
  * `dtype`; grad_weight (may be NULL) F32 or dtype.  grad_in may also be grad_out or hidden itself.  grad_in is the gradient of `in` and of `residual` alike.
- * Sums are f32 in a fixed order.  Workspace: mi355_rms_norm_grad_workspace_bytes, caller-owned; unused (may be NULL) when grad_weight is. */
+ * At most 2^31 columns.  Sums are f32 in a fixed order.  Workspace: mi355_rms_norm_grad_workspace_bytes, caller-owned; unused (may be NULL) when grad_weight is. */
 typedef struct {
     int64_t rows, cols;
     int64_t ld_out, ld_hidden, ld_in, ld_stream;                /* grad_out, hidden, grad_in, grad_hidden */

@@ -1,11 +1,17 @@
 """Calls that the operators around a linear layer once answered wrongly, or accepted and should not have, without a device: the host side on
 the fake HIP runtime, as in tests/test_linear_ops_cpu.py.  Their GPU side is tests/test_gpu_linear_ops_mends.py."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
 import numpy as np
 import pytest
 
 from cubecl_amd import ElemType, ops
+from cubecl_amd import _native as N
 from test_linear_ops_cpu import client, lib, log, make, refused  # noqa: F401
 
+ROOT = Path(__file__).resolve().parents[1]
 F32, BF16, F16, E4M3, UE8M0 = ElemType.F32, ElemType.BF16, ElemType.F16, ElemType.F8E4M3, ElemType.UE8M0
 
 
@@ -42,3 +48,54 @@ def test_gradients_of_shared_operands_over_an_empty_batch_are_written(client, mo
     a, b, da, db = make(client, (4, 5)), make(client, (5, 6)), make(client, (4, 5)), make(client, (5, 6))
     ops.matmul_fused_backward(client, g, None, d, lhs=a, rhs=b, grad_lhs=da, grad_rhs=db)
     assert done == [((4, 0), (0, 5), (4, 5), None), ((4, 5), (4, 5)), ((5, 0), (0, 6), (5, 6), None), ((5, 6), (5, 6))]
+
+
+# ---- launch limits ------------------------------------------------------------------------------------------------------------------
+GEOMETRY = r"""
+#include "../../cubecl_amd/csrc/linear_ops.hpp"
+#include <cstdio>
+using namespace mi355;
+int main()
+{
+    for (int64_t cols : {1ll, 63ll, 64ll, 65ll, 1ll << 20, (1ll << 27) - 1, 1ll << 27, (1ll << 27) + 1, 1ll << 28, (1ll << 30) + 7, 1ll << 31})
+        for (int64_t batch : {1ll, 2ll, 65535ll, 70000ll}) {
+            int64_t done = 0;
+            each_fold_launch(cols, batch, [&](int64_t c, int64_t wide, int64_t b, int64_t entries) {
+                const int64_t here = std::min(wide * FOLD_COLS, cols - c);
+                if (wide * 1024 * entries >= 1ll << 32 || entries > 65535 || b + entries > batch || c + (wide - 1) * FOLD_COLS >= cols) printf("fold %lld %lld\n", (long long)cols, (long long)batch);
+                done += here * entries;
+            });
+            if (done != cols * batch) printf("fold covers %lld of %lld x %lld\n", (long long)done, (long long)cols, (long long)batch);
+        }
+    for (int64_t cols : {1ll, 512ll, 16385ll, 1ll << 27, 1ll << 29, (long long)GRAD_MAX_COLS})
+        for (int64_t rows : {1ll, 3ll, 600ll, 1ll << 20}) {
+            const row_shape sh = grad_shape_for(rows, cols);
+            const int64_t wgs = norm_grad_partials(rows, cols), threads = sh.threads ? std::max(sh.threads, 256) * wgs : (cols + 2047) / 2048 * 256 * wgs;
+            if (wgs < 1 || wgs > rows || threads >= 1ll << 32) printf("grad %lld %lld\n", (long long)rows, (long long)cols);
+            if (sh.threads && (int64_t)sh.threads * sh.pieces * 8 < cols) printf("shape %lld %lld\n", (long long)rows, (long long)cols);
+            const row_shape f = shape_for(rows, cols);
+            if (f.threads && (int64_t)f.threads * f.pieces * 8 < cols) printf("forward shape %lld %lld\n", (long long)rows, (long long)cols);
+        }
+    for (int64_t cols = 1; cols <= 16384; ++cols)          // every row length that registers hold is held
+        for (int64_t rows : {1ll, 512ll, 513ll}) {
+            const row_shape f = shape_for(rows, cols), g = grad_shape_for(rows, cols);
+            if ((int64_t)f.threads * f.pieces * 8 < cols || (int64_t)g.threads * g.pieces * 8 < cols) printf("registers %lld\n", (long long)cols);
+        }
+    puts("done");
+}
+"""
+
+
+def test_launches_stay_below_the_thread_limit_and_cover_every_column(tmp_path):
+    src, exe = tmp_path / "geometry.cpp", tmp_path / "geometry"
+    src.write_text(GEOMETRY.replace("../../cubecl_amd", str(ROOT / "cubecl_amd")))
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", str(ROOT / "tests" / "fake_hip"), "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "done\n"
+
+
+def test_norm_gradient_refuses_more_columns_than_its_launches_hold(client):  # noqa: F811
+    need, d = C.c_uint64(), N.RmsNormGradDesc(rows=1, cols=(1 << 31) + 1, ld_out=1 << 32, ld_hidden=1 << 32, ld_in=1 << 32, dtype=BF16, dtype_weight=BF16, dtype_grad_weight=F32)
+    assert client.lib.mi355_rms_norm_grad_workspace_bytes(C.byref(d), C.byref(need)) == N.E_INVALID_ARGUMENT
+    p = make(client, (64,)).device_ptr()
+    assert client.lib.mi355_rms_norm_grad(client.ctx, None, C.byref(d), p, p, None, p, None, p, None, None, 0) == N.E_INVALID_ARGUMENT
+    assert log(client)["norm_grad"] == 0

@@ -5,35 +5,11 @@
 #include <vector>
 
 #include "linear_ops.hpp"
+#include "row_span.hpp"
 
 using namespace mi355;
 
 namespace {
-
-// ---- host: do two strided row sets share memory? ---------------------------------------------------------------------------------------
-struct row_span {
-    uintptr_t at;             // first byte
-    uint64_t rows, row_bytes, ld_bytes;
-    bool empty() const { return rows == 0 || row_bytes == 0; }
-    uintptr_t end() const { return at + (rows - 1) * ld_bytes + row_bytes; }
-};
-inline row_span span_of(const void *p, int64_t rows, int64_t cols, int64_t ld, int64_t esz)
-{
-    return {reinterpret_cast<uintptr_t>(p), (uint64_t)rows, (uint64_t)(cols * esz), (uint64_t)(ld * esz)};
-}
-enum { SPANS_APART = 0, SPANS_SAME = 1, SPANS_OVERLAP = 2 };
-inline int spans_relation(const row_span &a, const row_span &b)
-{
-    if (!a.at || !b.at || a.empty() || b.empty()) return SPANS_APART;
-    if (a.end() <= b.at || b.end() <= a.at) return SPANS_APART;
-    if (a.at == b.at && a.rows == b.rows && a.row_bytes == b.row_bytes && (a.rows == 1 || a.ld_bytes == b.ld_bytes)) return SPANS_SAME;
-    // column ranges of the same wider rows: apart where the one's columns end before the other's begin
-    if (a.ld_bytes == b.ld_bytes && a.ld_bytes) {
-        const uint64_t ld = a.ld_bytes, d = b.at >= a.at ? (b.at - a.at) % ld : (ld - (a.at - b.at) % ld) % ld;     // b's column, seen from a's
-        if (d >= a.row_bytes && d + b.row_bytes <= ld) return SPANS_APART;
-    }
-    return SPANS_OVERLAP;
-}
 
 bool float_type(int32_t t) { return t == MI355_DTYPE_F32 || t == MI355_DTYPE_BF16 || t == MI355_DTYPE_F16; }
 
@@ -63,15 +39,6 @@ uint64_t grad_bytes(const mi355_gemm_fused_grad_desc &d)
     return d.m && d.n && d.batch ? (uint64_t)(d.batch * slab_count(d)) * (uint64_t)d.n * sizeof(float) : 0;
 }
 
-// the whole batch as one set of rows, where its entries follow each other at their rows' distance; {0} where they do not
-row_span batch_span(const void *p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int64_t esz)
-{
-    if (batch == 1) return span_of(p, rows, cols, ld, esz);
-    if (stride == rows * ld) return span_of(p, batch * rows, cols, ld, esz);
-    if (stride >= (rows - 1) * ld + cols) return {reinterpret_cast<uintptr_t>(p), (uint64_t)batch, (uint64_t)(((rows - 1) * ld + cols) * esz), (uint64_t)(stride * esz)};
-    return {0, 0, 0, 0};
-}
-
 }  // namespace
 
 namespace mi355 {
@@ -88,29 +55,28 @@ int32_t validate_epilogue(mi355_ctx *ctx, const mi355_gemm_desc &d, const mi355_
     if (ep.stride_bias < 0 || ep.inc_row_scale < 0 || ep.stride_row_scale < 0 || ep.inc_col_scale < 0 || ep.stride_col_scale < 0 ||
         (ep.residual && ep.stride_residual < 0))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused: negative stride");
-    if (ep.pre && d.batch > 1 && ep.stride_pre < (d.m - 1) * ep.ld_pre + d.n)
+    if (ep.pre && !entries_apart(d.batch, d.m, d.n, ep.ld_pre, ep.stride_pre))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused: batch entries of the pre-activation overlap");
     const int64_t ec = (int64_t)dtype_size(d.dtype_c), ea = (int64_t)dtype_size(d.dtype_ab), eb = ep.bias ? (int64_t)dtype_size(ep.dtype_bias) : 1;
     if ((reinterpret_cast<uintptr_t>(ep.residual) | reinterpret_cast<uintptr_t>(ep.pre)) & (uintptr_t)(ec - 1) ||
         (reinterpret_cast<uintptr_t>(ep.bias) & (uintptr_t)(eb - 1)) ||
         ((reinterpret_cast<uintptr_t>(ep.row_scale) | reinterpret_cast<uintptr_t>(ep.col_scale)) & 3u))
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: an operand of the epilogue is not aligned to its element");
-    auto vec = [&](const void *p, int64_t count, int64_t inc, int64_t stride, int64_t esz) {      // from the first to the last element
-        return row_span{reinterpret_cast<uintptr_t>(p), 1, (uint64_t)(((count - 1) * inc + (d.batch - 1) * stride + 1) * esz), 0};
+    const row_span out = span_of(c, d.m, d.n, d.ldc, ec, d.batch, d.stride_c), pre = span_of(ep.pre, d.m, d.n, ep.ld_pre, ec, d.batch, ep.stride_pre);
+    const row_span res = span_of(ep.residual, d.m, d.n, ep.ld_residual, ec, d.batch, ep.stride_residual);
+    auto vec = [&](const void *p, int64_t count, int64_t inc, int64_t stride) {
+        return inc == 1 ? span_of(p, 1, count, 0, 4, d.batch, stride) : span_of(p, count, 1, inc, 4, d.batch, stride);
     };
-    const row_span out = batch_span(c, d.batch, d.m, d.n, d.ldc, d.stride_c, ec), pre = batch_span(ep.pre, d.batch, d.m, d.n, ep.ld_pre, ep.stride_pre, ec);
-    const row_span res = batch_span(ep.residual, ep.stride_residual ? d.batch : 1, d.m, d.n, ep.ld_residual, ep.stride_residual, ec);
-    const row_span none{0, 0, 0, 0};
     const row_span reads[] = {
-        d.k ? batch_span(a, d.stride_a ? d.batch : 1, d.trans_a ? d.k : d.m, d.trans_a ? d.m : d.k, d.lda, d.stride_a, ea) : none,
-        d.k ? batch_span(b, d.stride_b ? d.batch : 1, d.trans_b ? d.n : d.k, d.trans_b ? d.k : d.n, d.ldb, d.stride_b, ea) : none,
-        ep.bias ? vec(ep.bias, d.n, 1, ep.stride_bias, eb) : none, ep.row_scale ? vec(ep.row_scale, d.m, ep.inc_row_scale, ep.stride_row_scale, 4) : none,
-        ep.col_scale ? vec(ep.col_scale, d.n, ep.inc_col_scale, ep.stride_col_scale, 4) : none};
+        d.k ? span_of(a, d.trans_a ? d.k : d.m, d.trans_a ? d.m : d.k, d.lda, ea, d.batch, d.stride_a) : NO_SPAN,
+        d.k ? span_of(b, d.trans_b ? d.n : d.k, d.trans_b ? d.k : d.n, d.ldb, ea, d.batch, d.stride_b) : NO_SPAN,
+        span_of(ep.bias, 1, d.n, 0, eb, d.batch, ep.stride_bias), vec(ep.row_scale, d.m, ep.inc_row_scale, ep.stride_row_scale),
+        vec(ep.col_scale, d.n, ep.inc_col_scale, ep.stride_col_scale)};
     for (const row_span &r : reads)
         if (spans_relation(out, r) != SPANS_APART || spans_relation(pre, r) != SPANS_APART)
             return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: an output overlaps an operand");
     const int at = spans_relation(out, res);
-    if (at == SPANS_OVERLAP || (at == SPANS_SAME && d.batch > 1 && ep.stride_residual != d.stride_c))
+    if (at == SPANS_OVERLAP || (at == SPANS_SAME && d.batch > 1 && ep.stride_residual != d.stride_c))      // (the same bytes, entries and rows exchanged)
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: the residual overlaps the output without being it");
     if (spans_relation(pre, res) != SPANS_APART || spans_relation(pre, out) != SPANS_APART)
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused: the pre-activation overlaps the output or the residual");
@@ -151,7 +117,7 @@ MI355_API int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, con
     const bool reads_pre = d.activation != MI355_ACT_NONE;
     if (d.ld_out < d.n || (reads_pre && d.ld_pre < d.n) || (grad_pre && d.ld_grad < d.n))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused_grad: a leading dimension is smaller than the row");
-    if (d.batch > 1 && (d.stride_out < 0 || (reads_pre && d.stride_pre < 0) || (grad_pre && d.stride_grad < (d.m - 1) * d.ld_grad + d.n)))
+    if (d.batch > 1 && (d.stride_out < 0 || (reads_pre && d.stride_pre < 0) || (grad_pre && !entries_apart(d.batch, d.m, d.n, d.ld_grad, d.stride_grad))))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused_grad: a batch stride is negative, or entries of grad_pre overlap");
     const uint64_t need = grad_bias ? grad_bytes(d) : 0;
     if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3)))
@@ -159,15 +125,14 @@ MI355_API int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, con
     {
         const int64_t es = (int64_t)dtype_size(d.dtype);
         const int64_t bias_len = d.n * (d.batch_bias ? d.batch : 1);
-        const row_span reads[] = {batch_span(grad_out, d.stride_out ? d.batch : 1, d.m, d.n, d.ld_out, d.stride_out, es),
-                                  reads_pre ? batch_span(pre, d.stride_pre ? d.batch : 1, d.m, d.n, d.ld_pre, d.stride_pre, es) : row_span{0, 0, 0, 0}};
-        const row_span writes[] = {batch_span(grad_pre, d.batch, d.m, d.n, d.ld_grad, d.stride_grad, es),
-                                   grad_bias ? span_of(grad_bias, 1, bias_len, bias_len, (int64_t)dtype_size(d.dtype_bias)) : row_span{0, 0, 0, 0},
-                                   need ? row_span{reinterpret_cast<uintptr_t>(workspace), 1, need, need} : row_span{0, 0, 0, 0}};
+        const row_span reads[] = {span_of(grad_out, d.m, d.n, d.ld_out, es, d.batch, d.stride_out), reads_pre ? span_of(pre, d.m, d.n, d.ld_pre, es, d.batch, d.stride_pre) : NO_SPAN};
+        const row_span writes[] = {span_of(grad_pre, d.m, d.n, d.ld_grad, es, d.batch, d.stride_grad), span_of(grad_bias, 1, bias_len, 0, (int64_t)dtype_size(d.dtype_bias)),
+                                   span_of(need ? workspace : nullptr, 1, (int64_t)need, 0, 1)};
+        const int64_t read_stride[] = {d.stride_out, d.stride_pre};
         for (int w = 0; w < 3; ++w) {
             for (int r = 0; r < 2; ++r) {
                 const int rel = spans_relation(writes[w], reads[r]);
-                if (rel == SPANS_OVERLAP || (rel == SPANS_SAME && w != 0))
+                if (rel == SPANS_OVERLAP || (rel == SPANS_SAME && (w != 0 || (d.batch > 1 && read_stride[r] != d.stride_grad))))
                     return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: an output overlaps an operand");
             }
             for (int v = 0; v < w; ++v)
@@ -276,7 +241,7 @@ MI355_API int32_t mi355_rms_norm_grad(mi355_ctx *ctx, mi355_stream stream, const
                                   span_of(weight, 1, d.cols, d.cols, (int64_t)dtype_size(d.dtype_weight))};
         const row_span writes[] = {span_of(grad_in, d.rows, d.cols, d.ld_in, es),
                                    span_of(grad_weight, 1, d.cols, d.cols, (int64_t)dtype_size(d.dtype_grad_weight)),
-                                   grad_weight ? span_of(workspace, 1, (int64_t)(need / 4), (int64_t)(need / 4), 4) : row_span{0, 0, 0, 0}};
+                                   span_of(grad_weight ? workspace : nullptr, 1, (int64_t)(need / 4), 0, 4)};
         for (int w = 0; w < 3; ++w) {
             for (int r = 0; r < 5; ++r) {
                 const int rel = spans_relation(writes[w], reads[r]);

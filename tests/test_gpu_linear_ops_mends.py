@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from cubecl_amd import TensorHandle, ops
-from test_gpu_linear_ops import BF16, F32, close, down, empty, rand, rng, rounded, up
+from test_gpu_linear_ops import BF16, F32, act64, act_tol, close, down, empty, grad_tol, rand, rng, rounded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,29 @@ def test_gradients_of_shared_operands_over_an_empty_batch(client, dt):
         ops.matmul_fused_backward(client, empty(client, (0, 4, 6), dt), None, empty(client, (0, 4, 6), dt), grad_bias=bias,
                                   lhs=one(*lhs_shape) if lhs_shape[0] else empty(client, lhs_shape, dt), rhs=one(5, 6), grad_lhs=da, grad_rhs=db)
         assert all(bool((down(client, t) == 0).all()) for t in (da, db, bias))
+
+
+@pytest.mark.parametrize("m,n,k,batch", [(4, 8, 16, 3), (70, 33, 20, 4), (130, 264, 64, 2), (1, 40, 64, 5)])
+@pytest.mark.parametrize("dt", [F32, BF16], ids=lambda d: d.name)
+def test_entries_that_take_turns_by_rows(client, m, n, k, batch, dt):
+    """The kept argument, the residual and the gradients as [m][batch][n] parts of one [m][batch][4 n] tensor; the fourth part stays as it was."""
+    g = rng(81)
+    a, b, r, dy = rand(g, batch, m, k, dt=dt), rand(g, k, n, dt=dt, scale=k ** -0.5), rand(g, batch, m, n, dt=dt), rand(g, batch, m, n, dt=dt)
+    host = torch.full((m, batch, 4 * n), 7.0).to(r.dtype)
+    host[:, :, n: 2 * n], host[:, :, 2 * n: 3 * n] = r.transpose(0, 1), dy.transpose(0, 1)
+    whole = up(client, host)
+    part = lambda i: TensorHandle.new(whole.handle.offset_start_by(i * n * dt.size()), (batch, m, n), (4 * n, 4 * n * batch, 1), dt)
+    out, db = empty(client, (batch, m, n), dt), empty(client, (n,), F32)
+    ops.matmul_fused(client, up(client, a), up(client, b), out, activation="silu", residual=part(1), pre_activation=part(0))
+    z = a.double() @ b.double()
+    tol = 1e-5 * (a.double().abs() @ b.double().abs()) + 2.0 ** -22 * z.abs()
+    y = act64("silu", z)[0] + r.double()
+    close(down(client, out), y, rounded(y, act_tol("silu", z, tol) + 2.0 ** -22 * y.abs(), dt))
+    kept = down(client, part(0))
+    close(kept, z, rounded(z, tol, dt))
+    ops.matmul_fused_backward(client, part(2), part(0), part(2), activation="silu", grad_bias=db)
+    ref = dy.double() * act64("silu", kept)[1]
+    off = grad_tol("silu", kept, dy.double(), 2.0 ** -23 * ref.abs())
+    close(down(client, part(2)), ref, rounded(ref, off, dt))
+    close(down(client, db), ref.sum((0, 1)), off.sum((0, 1)) + 2.0 ** -24 * 512 * ref.abs().sum((0, 1)))
+    assert torch.equal(down(client, part(1)), r.double()) and bool((down(client, part(3)) == 7).all())

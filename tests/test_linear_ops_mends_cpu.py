@@ -7,7 +7,7 @@ from pathlib import Path
 import numpy as np
 import pytest
 
-from cubecl_amd import ElemType, ops
+from cubecl_amd import ElemType, TensorHandle, ops
 from cubecl_amd import _native as N
 from test_linear_ops_cpu import client, lib, log, make, refused  # noqa: F401
 
@@ -99,3 +99,108 @@ def test_norm_gradient_refuses_more_columns_than_its_launches_hold(client):  # n
     p = make(client, (64,)).device_ptr()
     assert client.lib.mi355_rms_norm_grad(client.ctx, None, C.byref(d), p, p, None, p, None, p, None, None, 0) == N.E_INVALID_ARGUMENT
     assert log(client)["norm_grad"] == 0
+
+
+# ---- which calls share memory -------------------------------------------------------------------------------------------------------
+SPANS = r"""
+#include "ROOT/cubecl_amd/csrc/row_span.hpp"
+#include <cstdio>
+#include <random>
+#include <vector>
+using namespace mi355;
+struct set { int64_t at, rows, cols, ld, batch, stride; };
+static char base[1];
+static std::vector<char> bytes(const set &s, int64_t esz)
+{
+    std::vector<char> v(4096, 0);
+    for (int64_t b = 0; b < s.batch; ++b)
+        for (int64_t r = 0; r < s.rows; ++r)
+            for (int64_t k = 0; k < s.cols * esz; ++k) v[s.at + (b * s.stride + r * s.ld) * esz + k] = 1;
+    return v;
+}
+int main()
+{
+    std::mt19937 g(7);
+    auto upto = [&](int64_t lo, int64_t hi) { return lo + (int64_t)(g() % (uint64_t)(hi - lo + 1)); };
+    int apart = 0, exact = 0, same = 0;
+    for (int t = 0; t < 200000; ++t) {
+        const int64_t esz = 1 << upto(0, 2), ld = upto(1, 12), stride = upto(0, 40);
+        auto one = [&](bool alike) {
+            set s{upto(0, 60), upto(0, 4), upto(0, 5), alike ? ld : upto(0, 12), upto(0, 3), alike ? stride : upto(0, 40)};
+            if (alike && t % 3 == 0) std::swap(s.ld, s.stride);
+            return s;
+        };
+        const bool alike = t & 1;
+        const set a = one(alike), b = t % 16 == 3 ? a : one(alike);
+        const row_span x = span_of(base + a.at, a.rows, a.cols, a.ld, esz, a.batch, a.stride), y = span_of(base + b.at, b.rows, b.cols, b.ld, esz, b.batch, b.stride);
+        const std::vector<char> p = bytes(a, esz), q = bytes(b, esz);
+        bool meet = false, equal = p == q;
+        for (size_t i = 0; i < p.size(); ++i) meet = meet || (p[i] && q[i]);
+        const int rel = spans_relation(x, y);
+        if (meet && rel == SPANS_APART) { puts("a shared byte was missed"); return 0; }
+        if (rel == SPANS_SAME && !equal) { puts("not the same bytes"); return 0; }
+        if (alike && !meet && rel != SPANS_APART) { puts("apart, and taken as overlapping"); return 0; }
+        if (spans_relation(y, x) != rel) { puts("one way is not the other"); return 0; }
+        apart += rel == SPANS_APART && x.row_bytes && y.row_bytes; exact += alike && !meet; same += rel == SPANS_SAME;
+    }
+    printf(apart > 1000 && exact > 1000 && same > 1000 ? "done\n" : "too few of a kind: %d %d %d\n", apart, exact, same);
+}
+"""
+
+
+def test_shared_bytes_are_seen_in_random_row_sets(tmp_path):
+    """Against the bytes themselves: no overlap is missed, and sets that step by the same distances are told apart exactly."""
+    src, exe = tmp_path / "spans.cpp", tmp_path / "spans"
+    src.write_text(SPANS.replace("ROOT", str(ROOT)))
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "done\n"
+
+
+def in_turn(client, handle, m, n, batch, dt=F32, at=0, width=None):  # noqa: F811
+    """[batch, m, n] stored [m][batch][width]."""
+    width = width or n
+    return TensorHandle.new(handle.offset_start_by(at * dt.size()), (batch, m, n), (width, batch * width, 1), dt)
+
+
+def test_outputs_on_interleaved_operands_are_refused(client):  # noqa: F811
+    m, n, k, batch = 4, 8, 8, 3
+    buf = client.empty(4 * (m * n * batch + 64))
+    lhs, rhs, out = in_turn(client, buf, m, k, batch), make(client, (k, n)), make(client, (batch, m, n))
+    # (the C entry: ops.matmul_fused copies such an lhs first)
+    d = N.GemmDesc(m=m, n=n, k=k, batch=batch, lda=batch * k, ldb=n, ldc=n, stride_a=k, stride_c=m * n, dtype_ab=F32, dtype_c=F32)
+    call = lambda c: client.lib.mi355_gemm_fused(client.ctx, None, C.byref(d), C.byref(N.GemmEpilogue()), lhs.device_ptr(), rhs.device_ptr(), c)      # noqa: E731
+    assert call(out.device_ptr()) == N.OK
+    assert [call(buf.offset_start_by(at).device_ptr()) for at in (0, 8, 4 * n)] == [N.E_INVALID_ARGUMENT] * 3
+    refused(ops.matmul_fused, client, make(client, (batch, m, k)), rhs, out, residual=in_turn(client, out.handle, m, n, batch), match="overlaps")
+    refused(ops.matmul_fused, client, make(client, (batch, m, k)), rhs, out, residual=lhs, pre_activation=in_turn(client, buf, m, n, batch, at=4), match="overlaps")
+    log(client, clear=True)
+    # the gradient's pass: in place is in place, anything else on its operands is not
+    g = in_turn(client, buf, m, n, batch)
+    ops.matmul_fused_backward(client, g, None, g)
+    refused(ops.matmul_fused_backward, client, g, None, in_turn(client, buf, m, n, batch, at=2), match="overlaps")
+    refused(ops.matmul_fused_backward, client, g, None, make(client, (batch, m, n), F32, None, buf), match="overlaps")
+    square = client.empty(4 * 3 * 3 * n)
+    a, b = make(client, (3, 3, n), F32, None, square), in_turn(client, square, 3, n, 3)
+    refused(ops.matmul_fused_backward, client, a, None, b, match="overlaps")      # the same bytes, entries and rows exchanged
+    assert log(client)["fused_grad"] == 1
+
+
+def test_interleaved_entries_and_parts_of_one_tensor_are_taken(client):  # noqa: F811
+    m, n, k, batch = 4, 8, 5, 3
+    a, b, out = make(client, (batch, m, k)), make(client, (k, n)), make(client, (batch, m, n))
+    whole = client.empty(4 * m * batch * 3 * n)
+    q, r, s = (in_turn(client, whole, m, n, batch, at=i * n, width=3 * n) for i in range(3))
+    ops.matmul_fused(client, a, b, out, activation="silu", pre_activation=in_turn(client, client.empty(4 * m * n * batch), m, n, batch))
+    ops.matmul_fused(client, a, b, out, activation="silu", pre_activation=q, residual=r)
+    ops.matmul_fused_backward(client, q, r, s, activation="silu")
+    ops.matmul_fused_backward(client, q, r, r, activation="silu")
+    # a column of scales beside an output in the same rows
+    wide = client.empty(4 * m * (n + 1))
+    ops.matmul_fused(client, make(client, (m, k)), b, make(client, (m, n), F32, (n + 1, 1), wide), lhs_scale=make(client, (m,), F32, (n + 1,), wide.offset_start_by(4 * n)))
+    assert log(client)["epilogue"] == 3 and log(client)["fused_grad"] == 2
+    refused(ops.matmul_fused, client, make(client, (m, k)), b, make(client, (m, n), F32, (n + 1, 1), wide),
+            lhs_scale=make(client, (m,), F32, (n + 1,), wide.offset_start_by(4 * n - 4)), match="overlaps")
+    # entries that do share memory
+    for stride, ld in ((n - 1, batch * n), (n, batch * n - 1), (0, n)):
+        refused(ops.matmul_fused, client, a, b, out, pre_activation=make(client, (batch, m, n), F32, (stride, ld, 1)), code=N.E_UNSUPPORTED_STRIDES)
+        refused(ops.matmul_fused_backward, client, out, None, make(client, (batch, m, n), F32, (stride, ld, 1)), code=N.E_UNSUPPORTED_STRIDES)

@@ -2,6 +2,7 @@
 // epilogue, mi355_global_norm and mi355_clip_by_global_norm.  What a call may not ask for is refused here, before anything is launched.
 #include <cfloat>
 #include <cmath>
+#include <initializer_list>
 #include <vector>
 
 #include "linear_ops.hpp"
@@ -10,6 +11,13 @@
 using namespace mi355;
 
 namespace {
+
+// every pointer of a call against the size of what it points to
+struct operand { const void *p; int64_t esz; };
+bool aligned(std::initializer_list<operand> ops)
+{
+    return std::all_of(ops.begin(), ops.end(), [](const operand &o) { return (reinterpret_cast<uintptr_t>(o.p) & (uintptr_t)(o.esz - 1)) == 0; });
+}
 
 bool float_type(int32_t t) { return t == MI355_DTYPE_F32 || t == MI355_DTYPE_BF16 || t == MI355_DTYPE_F16; }
 
@@ -106,6 +114,7 @@ MI355_API int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, con
     if (grad_bias && d.dtype_bias != MI355_DTYPE_F32 && d.dtype_bias != d.dtype)
         return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm_fused_grad: the bias gradient must be f32 or of the operands' type (got %d)", d.dtype_bias);
     if (d.n == 0) return MI355_OK;
+    if (!aligned({{grad_bias, (int64_t)dtype_size(d.dtype_bias)}})) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: grad_bias is not aligned to its element");
     hipStream_t s = stream_of(ctx, stream);
     if (d.m == 0 || d.batch == 0) {                                   // sums over no rows: zeros
         if (grad_bias && (d.batch || !d.batch_bias)) launch_fold_columns(s, nullptr, 0, d.n, d.batch_bias ? d.batch : 1, grad_bias, d.dtype_bias);
@@ -119,6 +128,11 @@ MI355_API int32_t mi355_gemm_fused_grad(mi355_ctx *ctx, mi355_stream stream, con
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused_grad: a leading dimension is smaller than the row");
     if (d.batch > 1 && (d.stride_out < 0 || (reads_pre && d.stride_pre < 0) || (grad_pre && !entries_apart(d.batch, d.m, d.n, d.ld_grad, d.stride_grad))))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_gemm_fused_grad: a batch stride is negative, or entries of grad_pre overlap");
+    {
+        const int64_t es = (int64_t)dtype_size(d.dtype);
+        if (!aligned({{grad_out, es}, {reads_pre ? pre : nullptr, es}, {grad_pre, es}}))
+            return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: an operand is not aligned to its element");
+    }
     const uint64_t need = grad_bias ? grad_bytes(d) : 0;
     if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3)))
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_gemm_fused_grad: the workspace has %llu of %llu bytes", (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -176,6 +190,8 @@ MI355_API int32_t mi355_rms_norm(mi355_ctx *ctx, mi355_stream stream, const mi35
         (f8 && d.scale_block && d.ld_scales < d.cols / 32))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_rms_norm: a row stride is smaller than the row");
     const int64_t es = (int64_t)dtype_size(d.dtype), eo = (int64_t)dtype_size(d.dtype_out);
+    if (!aligned({{in, es}, {residual, es}, {weight, (int64_t)dtype_size(d.dtype_weight)}, {hidden, es}, {out, eo}, {scales, d.scale_block ? 1 : 4}, {rstd, 4}}))
+        return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm: an operand is not aligned to its element");
     {
         const row_span reads[] = {span_of(in, d.rows, d.cols, d.ld_in, es), span_of(residual, d.rows, d.cols, d.ld_residual, es),
                                   span_of(weight, 1, d.cols, d.cols, (int64_t)dtype_size(d.dtype_weight))};
@@ -222,6 +238,7 @@ MI355_API int32_t mi355_rms_norm_grad(mi355_ctx *ctx, mi355_stream stream, const
         (grad_weight && d.dtype_grad_weight != MI355_DTYPE_F32 && d.dtype_grad_weight != d.dtype))
         return fail(ctx, MI355_E_UNSUPPORTED, "mi355_rms_norm_grad: the weight and its gradient must be f32 or of the operands' type");
     if (d.cols == 0) return MI355_OK;
+    if (!aligned({{grad_weight, (int64_t)dtype_size(d.dtype_grad_weight)}})) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: grad_weight is not aligned to its element");
     hipStream_t s = stream_of(ctx, stream);
     if (d.rows == 0) {
         if (grad_weight) launch_fold_columns(s, nullptr, 0, d.cols, 1, grad_weight, d.dtype_grad_weight);      // a sum over no rows: zeros
@@ -231,6 +248,11 @@ MI355_API int32_t mi355_rms_norm_grad(mi355_ctx *ctx, mi355_stream stream, const
     if (!grad_out || !hidden || !rstd || !grad_in) return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: NULL operand");
     if (d.ld_out < d.cols || d.ld_hidden < d.cols || d.ld_in < d.cols || (grad_hidden && d.ld_stream < d.cols))
         return fail(ctx, MI355_E_UNSUPPORTED_STRIDES, "mi355_rms_norm_grad: a row stride is smaller than the row");
+    {
+        const int64_t es = (int64_t)dtype_size(d.dtype);
+        if (!aligned({{grad_out, es}, {hidden, es}, {weight, (int64_t)dtype_size(d.dtype_weight)}, {rstd, 4}, {grad_hidden, es}, {grad_in, es}}))
+            return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: an operand is not aligned to its element");
+    }
     const uint64_t need = (uint64_t)norm_grad_partials(d.rows, d.cols) * (uint64_t)d.cols * sizeof(float);
     if (grad_weight && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3)))
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "mi355_rms_norm_grad: the workspace has %llu of %llu bytes", (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -355,6 +377,7 @@ int32_t run(mi355_ctx *ctx, mi355_stream stream, const char *what, const mi355_t
     if (!workspace || workspace_bytes < MAX_PARTIALS * sizeof(double) || (reinterpret_cast<uintptr_t>(workspace) & 7))
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "%s: the workspace has %llu of %llu bytes, or is not 8-byte aligned", what, (unsigned long long)workspace_bytes,
                     (unsigned long long)(MAX_PARTIALS * sizeof(double)));
+    if (!aligned({{out_norm, 4}})) return fail(ctx, MI355_E_INVALID_ARGUMENT, "%s: the norm is not aligned to its element", what);
     if (out && !outputs_apart(in, out, count))
         return fail(ctx, MI355_E_INVALID_ARGUMENT, "%s: an output overlaps another tensor of the list", what);
     {

@@ -904,8 +904,8 @@ def rms_norm_backward(client: ComputeClient, grad_output: TensorHandle, hidden: 
         if need.value:
             ws = client.empty(need.value)
     client._s.check(client.lib.mi355_rms_norm_grad(
-        client.ctx, client.on(g, h, weight, rstd, s, grad_input, grad_weight, ws), C.byref(desc), g.device_ptr(), h.device_ptr(),
-        _ptr(weight), rstd.device_ptr(), _ptr(s), grad_input.device_ptr(), _ptr(grad_weight), _ptr(ws), need.value))
+        client.ctx, client.on(g, h, weight, rstd, s, grad_input, grad_weight, ws), C.byref(desc), g.device_ptr(), _ptr(h),
+        _ptr(weight), _ptr(rstd), _ptr(s), grad_input.device_ptr(), _ptr(grad_weight), _ptr(ws), need.value))
 
 
 class TensorList:
@@ -947,7 +947,7 @@ def global_norm(client: ComputeClient, tensors, output: TensorHandle) -> None:
     _flat(output, (1,), (ElemType.F32,), "global_norm: output")
     ws = _norm_workspace(client)
     client._s.check(client.lib.mi355_global_norm(client.ctx, client.on(*tensors.memories, output, ws), tensors.spans, len(tensors),
-                                                 output.device_ptr(), ws.device_ptr(), ws.size))
+                                                 _ptr(output), ws.device_ptr(), ws.size))
 
 
 def clip_by_global_norm(client: ComputeClient, tensors, max_norm: float, *, outputs=None, total_norm: Optional[TensorHandle] = None) -> None:

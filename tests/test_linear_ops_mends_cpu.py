@@ -96,7 +96,8 @@ def test_launches_stay_below_the_thread_limit_and_cover_every_column(tmp_path):
 def test_norm_gradient_refuses_more_columns_than_its_launches_hold(client):  # noqa: F811
     need, d = C.c_uint64(), N.RmsNormGradDesc(rows=1, cols=(1 << 31) + 1, ld_out=1 << 32, ld_hidden=1 << 32, ld_in=1 << 32, dtype=BF16, dtype_weight=BF16, dtype_grad_weight=F32)
     assert client.lib.mi355_rms_norm_grad_workspace_bytes(C.byref(d), C.byref(need)) == N.E_INVALID_ARGUMENT
-    p = make(client, (64,)).device_ptr()
+    held = make(client, (64,))
+    p = held.device_ptr()
     assert client.lib.mi355_rms_norm_grad(client.ctx, None, C.byref(d), p, p, None, p, None, p, None, None, 0) == N.E_INVALID_ARGUMENT
     assert log(client)["norm_grad"] == 0
 
@@ -204,3 +205,44 @@ def test_interleaved_entries_and_parts_of_one_tensor_are_taken(client):  # noqa:
     for stride, ld in ((n - 1, batch * n), (n, batch * n - 1), (0, n)):
         refused(ops.matmul_fused, client, a, b, out, pre_activation=make(client, (batch, m, n), F32, (stride, ld, 1)), code=N.E_UNSUPPORTED_STRIDES)
         refused(ops.matmul_fused_backward, client, out, None, make(client, (batch, m, n), F32, (stride, ld, 1)), code=N.E_UNSUPPORTED_STRIDES)
+
+
+# ---- alignment and missing operands ---------------------------------------------------------------------------------------------------
+def test_pointers_off_their_element_are_refused(client):  # noqa: F811
+    """Each operand of the C entry points half an element off, the others as they should be; one element off is fine."""
+    held = [make(client, (64,), F32) for _ in range(8)]
+    p = [t.device_ptr() for t in held]
+    d = N.RmsNormDesc(rows=2, cols=8, ld_in=8, ld_residual=8, ld_hidden=8, ld_out=8, eps=1e-6, dtype=BF16, dtype_weight=F32, dtype_out=BF16)
+    norm = lambda off, d=d: client.lib.mi355_rms_norm(client.ctx, None, C.byref(d), *[x + o for x, o in zip(p, off)][:5], p[5] + off[5] if d.dtype_out == E4M3 else None, p[6] + off[6])      # noqa: E731
+    assert norm([2, 2, 4, 2, 2, 0, 4]) == N.OK
+    for i, o in enumerate((1, 1, 2, 1, 1, None, 2)):
+        assert o is None or norm([o if j == i else 0 for j in range(7)]) == N.E_INVALID_ARGUMENT, i
+    d8 = N.RmsNormDesc(rows=2, cols=8, ld_in=8, ld_residual=8, ld_hidden=8, ld_out=8, eps=1e-6, dtype=BF16, dtype_weight=F32, dtype_out=E4M3)
+    assert norm([0, 0, 0, 0, 1, 4, 0], d8) == N.OK and norm([0, 0, 0, 0, 1, 2, 0], d8) == N.E_INVALID_ARGUMENT
+    g = N.RmsNormGradDesc(rows=2, cols=8, ld_out=8, ld_hidden=8, ld_in=8, ld_stream=8, dtype=BF16, dtype_weight=F32, dtype_grad_weight=F32)
+    need = C.c_uint64()
+    assert client.lib.mi355_rms_norm_grad_workspace_bytes(C.byref(g), C.byref(need)) == N.OK
+    ws = client.empty(need.value)
+    grad = lambda off: client.lib.mi355_rms_norm_grad(client.ctx, None, C.byref(g), *[x + o for x, o in zip(p, off)], ws.device_ptr(), need.value)      # noqa: E731
+    assert grad([2, 2, 4, 4, 2, 2, 4]) == N.OK
+    for i, o in enumerate((1, 1, 2, 2, 1, 1, 2)):
+        assert grad([o if j == i else 0 for j in range(7)]) == N.E_INVALID_ARGUMENT, i
+    f = N.GemmFusedGradDesc(m=2, n=8, batch=1, ld_out=8, ld_pre=8, ld_grad=8, dtype=BF16, activation=N.ACT_SILU, dtype_bias=F32)
+    assert client.lib.mi355_gemm_fused_grad_workspace_bytes(C.byref(f), C.byref(need)) == N.OK
+    ws = client.empty(need.value)
+    fused = lambda off: client.lib.mi355_gemm_fused_grad(client.ctx, None, C.byref(f), *[x + o for x, o in zip(p, off)], ws.device_ptr(), need.value)      # noqa: E731
+    assert fused([2, 2, 2, 4]) == N.OK
+    for i, o in enumerate((1, 1, 1, 2)):
+        assert fused([o if j == i else 0 for j in range(4)]) == N.E_INVALID_ARGUMENT, i
+    spans, ws = ops.TensorList([make(client, (8,))]).spans, client.empty(1 << 16)
+    assert client.lib.mi355_global_norm(client.ctx, None, spans, 1, p[0] + 2, ws.device_ptr(), 1 << 16) == N.E_INVALID_ARGUMENT
+    got = log(client)
+    assert (got["norm"], got["norm_grad"], got["fused_grad"], got["sums"]) == (2, 1, 1, 0)
+
+
+def test_missing_operands_are_refused(client):  # noqa: F811
+    g, w, r, dx = make(client, (5, 64), F16), make(client, (64,), F16), make(client, (5,)), make(client, (5, 64), F16)
+    refused(ops.rms_norm_backward, client, g, g, w, None, dx, match="NULL")
+    refused(ops.rms_norm_backward, client, g, None, w, r, dx, match="NULL")
+    refused(ops.global_norm, client, [g], None, match="NULL")
+    assert log(client)["norm_grad"] == 0 and log(client)["sums"] == 0

@@ -146,8 +146,15 @@ scale_kernel(TABLE tab, const double *__restrict__ partial, uint32_t count, floa
     __shared__ double slot[4];
     const double norm = norm_of(partial, count, slot);
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) out_norm[0] = (float)norm;
-    // (an infinite or NaN norm: no factor brings it to max_norm)
-    const float coef = !(norm <= DBL_MAX) ? __uint_as_float(0x7FC00000u) : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.0f;
+    // (an infinite or NaN norm: no factor brings it to max_norm.)  A factor near the end of the f32 range, which a norm beyond that range asks for,
+    // would have few bits left: `down` is a power of two, half of its exponent, and `coef` the rest.  What x * down loses there is 0 in the end.
+    float coef = 1.0f, down = 1.0f;
+    if (!(norm <= DBL_MAX)) coef = __uint_as_float(0x7FC00000u);
+    else if (norm > (double)max_norm) {
+        const double f = (double)max_norm / norm, half = f < 0x1p-100 ? ldexp(1.0, ilogb(f) / 2) : 1.0;
+        down = (float)half;
+        coef = (float)(f / half);
+    }
     for (uint32_t k = blockIdx.x; k < tab.chunks; k += gridDim.x) {
         const chunk_place p = place_of(tab, k);
         if (coef == 1.0f && p.in == p.out) continue;              // in place and nothing to scale
@@ -155,7 +162,7 @@ scale_kernel(TABLE tab, const double *__restrict__ partial, uint32_t count, floa
             constexpr int DT = decltype(dt)::value;
             each_run<DT>(p, [&](float (&x)[8], int64_t o, int valid) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= coef;
+                for (int e = 0; e < 8; ++e) x[e] = x[e] * down * coef;
                 store8<DT, true>(p.out, o, valid, x);
             });
         };

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from cubecl_amd import TensorHandle, ops
-from test_gpu_linear_ops import BF16, F32, act64, act_tol, close, down, empty, grad_tol, rand, rng, rounded, up
+from test_gpu_linear_ops import BF16, F32, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, rng, rounded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,19 @@ def test_entries_that_take_turns_by_rows(client, m, n, k, batch, dt):
     close(down(client, part(2)), ref, rounded(ref, off, dt))
     close(down(client, db), ref.sum((0, 1)), off.sum((0, 1)) + 2.0 ** -24 * 512 * ref.abs().sum((0, 1)))
     assert torch.equal(down(client, part(1)), r.double()) and bool((down(client, part(3)) == 7).all())
+
+
+@pytest.mark.parametrize("max_norm", [1.0, 1e-3, 1e-20, 1e-38])
+def test_clip_by_factors_at_the_end_of_the_range(client, max_norm):
+    """Norms that f32 does not hold brought down to small ones: the factor is a subnormal f32, or none at all, the results are ordinary numbers.
+    Two roundings in f32 (the factor, the product) and the output's own; half a subnormal step of the type at the very end."""
+    g = rng(82)
+    for dt, scale in ((F32, 3e37), (BF16, 3e37), (F32, 1e25)):
+        parts = [rand(g, 5000, scale=scale).to(TORCH[dt]), rand(g, 33, 70, scale=scale * 1e-9).to(TORCH[dt])]
+        handles, total = [up(client, t) for t in parts], empty(client, (1,), F32)
+        ops.clip_by_global_norm(client, handles, max_norm, total_norm=total)
+        limit = float(torch.tensor(max_norm, dtype=torch.float32))
+        factor = limit / float(torch.sqrt(sum(t.double().square().sum() for t in parts)))
+        for t, h in zip(parts, handles):
+            ref = t.double() * factor
+            close(down(client, h), ref, rounded(ref, 2.0 ** -23 * 1.01 * ref.abs() + (2.0 ** -149 if dt == F32 else 2.0 ** -134), dt))

@@ -44,7 +44,8 @@ epilogue_kernel(const float *__restrict__ prod, uint32_t slabs, int64_t slab_str
         float v[8];
         const float rs = ep.p.row_scale ? ep.p.row_scale[b * ep.p.stride_row_scale + row * ep.p.inc_row_scale] : 1.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] *= rs * (ep.p.col_scale && e < valid ? ep.p.col_scale[b * ep.p.stride_col_scale + (i + e) * ep.p.inc_col_scale] : 1.0f);
+        for (int e = 0; e < 8; ++e)      // (one after the other, as on the accumulators: the scales' product may leave the range where the value does not)
+            z[e] = z[e] * rs * (ep.p.col_scale && e < valid ? ep.p.col_scale[b * ep.p.stride_col_scale + (i + e) * ep.p.inc_col_scale] : 1.0f);
         if (ep.p.bias) {
             load8_any(ep.p.bias, ep.p.dtype_bias, b * ep.p.stride_bias + i, valid, v);
 #pragma unroll

@@ -75,3 +75,18 @@ def test_clip_by_factors_at_the_end_of_the_range(client, max_norm):
         for t, h in zip(parts, handles):
             ref = t.double() * factor
             close(down(client, h), ref, rounded(ref, 2.0 ** -23 * 1.01 * ref.abs() + (2.0 ** -149 if dt == F32 else 2.0 ** -134), dt))
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 128, 64), (40, 64, 16384), (128, 256, 8192), (100, 100, 5001)])
+@pytest.mark.parametrize("dt", [BF16, F32], ids=lambda d: d.name)
+@pytest.mark.parametrize("power", [100, -100])
+def test_scales_whose_product_leaves_the_range(client, m, n, k, dt, power):
+    """(A B) rs cs with both scales 2^100 (2^-100) and products near 2^-80 (2^80): the same on one tile's accumulators and in the fold of K slices.
+    Powers of two, so the only error is the product's."""
+    g = rng(83)
+    side = 2.0 ** (-40 if power > 0 else 40)
+    a, b = rand(g, m, k, dt=dt, scale=side), rand(g, k, n, dt=dt, scale=side * k ** -0.5)
+    out, scale = empty(client, (m, n), F32), torch.full((max(m, n),), 2.0 ** power)
+    ops.matmul_fused(client, up(client, a), up(client, b.t().contiguous()).permute((1, 0)), out, lhs_scale=up(client, scale[:m]), rhs_scale=up(client, scale[:n]))
+    ref, whole = a.double() @ b.double(), 2.0 ** (2 * power)
+    close(down(client, out), ref * whole, 1e-5 * (a.double().abs() @ b.double().abs()) * whole)

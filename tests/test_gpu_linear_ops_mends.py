@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from cubecl_amd import TensorHandle, ops
-from test_gpu_linear_ops import BF16, F32, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, rng, rounded, up
+from test_gpu_linear_ops import BF16, E4M3, E5M2, F32, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, raw_down, rng, rounded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,20 @@ def test_scales_whose_product_leaves_the_range(client, m, n, k, dt, power):
     ops.matmul_fused(client, up(client, a), up(client, b.t().contiguous()).permute((1, 0)), out, lhs_scale=up(client, scale[:m]), rhs_scale=up(client, scale[:n]))
     ref, whole = a.double() @ b.double(), 2.0 ** (2 * power)
     close(down(client, out), ref * whole, 1e-5 * (a.double().abs() @ b.double().abs()) * whole)
+
+
+@pytest.mark.parametrize("rows,cols", [(4000, 1024), (1500, 4096), (400, 8192), (500, 16384), (300, 20000)])
+@pytest.mark.parametrize("out_dt", [E4M3, E5M2], ids=lambda d: d.name)
+def test_8_bit_rows_are_quotients(client, rows, cols, out_dt):
+    """Every 8-bit value is the nearest to y / scale of the kernel's own y (its f32 output) and scale, ties to even: a quotient that is a rounding
+    off falls on the other side of a tie in one of 2^19 values, and there are some 2^22."""
+    g = rng(84)
+    x, w = rand(g, rows, cols, dt=BF16), rand(g, cols, dt=F32, scale=2.0 ** -110)
+    w[: cols // 2] *= 2.0 ** 108                                        # ordinary rows, and from the third on rows of values near 2^-110
+    x[2::3, : cols // 2] = 0
+    x, w = up(client, x), up(client, w)
+    y, q, s = empty(client, (rows, cols), F32), empty(client, (rows, cols), out_dt), empty(client, (rows,), F32)
+    ops.rms_norm(client, x, w, y)
+    ops.rms_norm(client, x, w, q, scales=s)
+    want = (down(client, y).float() / down(client, s).float()[:, None]).to(TORCH[out_dt])
+    assert torch.equal(raw_down(client, q), want.view(torch.uint8).reshape(-1))

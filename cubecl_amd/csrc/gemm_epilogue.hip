@@ -13,6 +13,21 @@ using namespace mi355;
 
 namespace {
 
+template <bool WIDE>
+__device__ __forceinline__ void act8(const epilogue_args &ep, float (&z)[8])
+{
+    if (ep.kind == ACT_SIGMOID) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = act_sigmoid<WIDE>(z[e], ep.a, ep.b);
+    } else if (ep.kind == ACT_ERF) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = act_erf<WIDE>(z[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = act_linear(z[e], ep.floor);
+    }
+}
+
 // One run of eight columns a thread, runs counted along the rows (grid.x), batch entries in grid.y; slabs in fours, so that four loads fly.
 template <class INDEX>
 __global__ void __launch_bounds__(256)
@@ -52,16 +67,8 @@ epilogue_kernel(const float *__restrict__ prod, uint32_t slabs, int64_t slab_str
             for (int e = 0; e < 8; ++e) z[e] += v[e];
         }
         if (ep.p.pre) store8_any(ep.p.pre, ep.dtype_c, b * ep.p.stride_pre + row * ep.p.ld_pre + i, valid, z);
-        if (ep.kind == ACT_SIGMOID) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = act_sigmoid(z[e], ep.a, ep.b);
-        } else if (ep.kind == ACT_ERF) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = act_erf(z[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = act_linear(z[e], ep.floor);
-        }
+        if (ep.dtype_c == MI355_DTYPE_F32) act8<true>(ep, z);
+        else act8<false>(ep, z);
         if (ep.p.residual) {
             load8_any(ep.p.residual, ep.dtype_c, b * ep.p.stride_residual + row * ep.p.ld_residual + i, valid, v);
 #pragma unroll
@@ -95,7 +102,7 @@ fused_grad_kernel(fused_grad_args a)
             } else {
                 const vec8<DT> z = load8<DT>(a.pre, b * a.stride_pre + row * a.ld_pre + i, valid);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = get(g, e) * act_grad_of<ACT>(get(z, e));
+                for (int e = 0; e < 8; ++e) d[e] = get(g, e) * act_grad_of<ACT, DT == MI355_DTYPE_F32>(get(z, e));
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += d[e];

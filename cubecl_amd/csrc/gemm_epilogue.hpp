@@ -44,6 +44,12 @@ __device__ __forceinline__ const epilogue_args &epilogue_of()
     return *(const epilogue_args *)(const char *)p;
 }
 
+template <bool WIDE>
+__device__ __forceinline__ float activate(const epilogue_args &ep, float z)
+{
+    return ep.kind == ACT_SIGMOID ? act_sigmoid<WIDE>(z, ep.a, ep.b) : ep.kind == ACT_ERF ? act_erf<WIDE>(z) : act_linear(z, ep.floor);
+}
+
 // -> the value to store at (row, col) of batch entry b; `pre` is written here
 __device__ __forceinline__ float finish_one(const epilogue_args &ep, int64_t b, int64_t row, int64_t col, float v)
 {
@@ -51,7 +57,7 @@ __device__ __forceinline__ float finish_one(const epilogue_args &ep, int64_t b, 
     if (ep.p.col_scale) v *= ep.p.col_scale[b * ep.p.stride_col_scale + col * ep.p.inc_col_scale];
     if (ep.p.bias) v += load1_any(ep.p.bias, ep.p.dtype_bias, b * ep.p.stride_bias + col);
     if (ep.p.pre) store1_any(ep.p.pre, ep.dtype_c, b * ep.p.stride_pre + row * ep.p.ld_pre + col, v);
-    v = ep.kind == ACT_SIGMOID ? act_sigmoid(v, ep.a, ep.b) : ep.kind == ACT_ERF ? act_erf(v) : act_linear(v, ep.floor);
+    v = ep.dtype_c == MI355_DTYPE_F32 ? activate<true>(ep, v) : activate<false>(ep, v);
     if (ep.p.residual) v += load1_any(ep.p.residual, ep.dtype_c, b * ep.p.stride_residual + row * ep.p.ld_residual + col);
     return v;
 }
@@ -70,6 +76,7 @@ struct tile_finish {
     char *c;
     int valid;
     float bias[8], cs[8];
+    static constexpr bool WIDE = DT_C == MI355_DTYPE_F32;        // the activations' precision
     static constexpr bool BUFFERED = AHEAD && DT_C != MI355_DTYPE_F32;      // a second set of pieces (f32: the registers end)
     struct pieces { float rs[AHEAD ? PIECES : 1]; vec8<DT_C> res[AHEAD ? PIECES : 1]; } now, next;
 
@@ -116,7 +123,7 @@ struct tile_finish {
         if (ep.p.pre) store8<DT_C, true>(ep.p.pre, b * ep.p.stride_pre + r * ep.p.ld_pre + col, valid, z);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            z[e] = KIND == ACT_SIGMOID ? act_sigmoid(z[e], ep.a, ep.b) : KIND == ACT_ERF ? act_erf(z[e]) : act_linear(z[e], ep.floor);
+            z[e] = KIND == ACT_SIGMOID ? act_sigmoid<WIDE>(z[e], ep.a, ep.b) : KIND == ACT_ERF ? act_erf<WIDE>(z[e]) : act_linear(z[e], ep.floor);
             if (ep.p.residual) z[e] += get(now.res[slot], e);
         }
         store8<DT_C, true>(c, b * stride_c + r * ldc + col, valid, z);
@@ -140,7 +147,7 @@ struct tile_finish {
 #pragma unroll
         for (int it = 0; it < GROUP; ++it)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[it][e] = KIND == ACT_SIGMOID ? act_sigmoid(z[it][e], a, b) : KIND == ACT_ERF ? act_erf(z[it][e]) : act_linear(z[it][e], floor);
+            for (int e = 0; e < 8; ++e) z[it][e] = KIND == ACT_SIGMOID ? act_sigmoid<WIDE>(z[it][e], a, b) : KIND == ACT_ERF ? act_erf<WIDE>(z[it][e]) : act_linear(z[it][e], floor);
     }
     template <bool INSIDE>
     __device__ __forceinline__ void store_all(void *p, int64_t at_, int64_t ld, int64_t r0, const float (&z)[GROUP][8])

@@ -175,58 +175,136 @@ __device__ __forceinline__ V block_reduce(V v, V *slot, F f)
 }
 
 // ---- activations --------------------------------------------------------------------------------------------------------------------
-// exp through v_exp_f32 (2^x, 1 ulp): the product x * log2(e) is off by |x| 2^-24 relative, far below what 16-bit outputs show and 2^-21 of
-// the result for the |x| <= 8 that f32 outputs show.  1 / (1 + e) through v_rcp_f32 (1 ulp).
+// Two forms.  For 16-bit outputs: exp through v_exp_f32 (2^x, 1 ulp) of the rounded product x * log2(e), which is off by |x| 2^-24 relative, and
+// 1 / (1 + e) through v_rcp_f32 (1 ulp): below 2^-15 of the result wherever the type has a number for it.  WIDE, for f32 outputs: the exponent in
+// two pieces, so that the tails keep their bits (2^-20 of the result; a single one is off by 2^-20 at z = -10, 2^-18 at -80).
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
-// erfc(|x|) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p |x|): Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26,
-// absolute error 1.5e-7; the factor exp(-x^2) keeps the left tail of gelu free of cancellation.
-__device__ __forceinline__ float erfc_abs(float x, float exp_neg_x2)
-{
-    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
-    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    return p * exp_neg_x2;
-}
 // z limited to [lo, hi]; a NaN stays
 __device__ __forceinline__ float limit(float z, float lo, float hi) { return z < lo ? lo : (z > hi ? hi : z); }
 
+// (Pieces of a product stay apart only while the compiler leaves the product alone: contraction is off where one is split.)
+// 2^-(hi + lo), lo the few bits that hi has no room for; results below the normal numbers included
+__device__ __forceinline__ float exp2_neg(float hi, float lo)
+{
+    asm("" : "+v"(hi));      // (rounded: exp2f adds 64 to what is below the normal numbers, and that sum would take hi's product in, and lo with it twice)
+    const float e = exp2f(-hi);
+    return __builtin_fmaf(e, lo * -0.693147182f, e);
+}
+// 1 / d, v_rcp_f32 and one Newton step: within 0.6 ulp for the d of [1, 8] met here
+__device__ __forceinline__ float rcp_of(float d)
+{
+    const float r = __builtin_amdgcn_rcpf(d);
+    return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
+// |u| log2(e) of silu (u = z) and of gelu's tanh form (u = 2 C0 z (1 + C1 z^2)) in two pieces, for 0 <= w = |z| limited
+struct exponent { float hi, lo; };
+__device__ __forceinline__ exponent silu_exponent(float w)
+{
+#pragma clang fp contract(off)
+    constexpr float L = 1.44269502f, L_LO = 1.92596303e-08f;       // log2(e)
+    const float hi = w * L;
+    return {hi, __builtin_fmaf(w, L_LO, __builtin_fmaf(w, L, -hi))};
+}
+__device__ __forceinline__ exponent gelu_tanh_exponent(float w)
+{
+#pragma clang fp contract(off)
+    constexpr float A = 2.30220819f, A_LO = 1.29484024e-08f, B = 0.102943242f, B_LO = -2.01619832e-09f;      // 2 C0 log2(e) and its product with C1
+    const float q = w * w, q_lo = __builtin_fmaf(w, w, -q);
+    const float m = B * q, m_lo = __builtin_fmaf(B, q_lo, __builtin_fmaf(B_LO, q, __builtin_fmaf(B, q, -m)));
+    const float s = A + m, part = s - A, s_lo = (A - (s - part)) + (m - part) + m_lo + A_LO;
+    const float hi = w * s;
+    return {hi, __builtin_fmaf(w, s_lo, __builtin_fmaf(w, s, -hi))};
+}
+// sigmoid(u) and 1 - sigmoid(u) from |u| log2(e), each with all its bits
+struct sigmoid_pair { float s, c; };
+__device__ __forceinline__ sigmoid_pair sigmoid_both(bool negative, exponent x)
+{
+    const float e = exp2_neg(x.hi, x.lo), r = rcp_of(1.0f + e), small_ = e * r;
+    return negative ? sigmoid_pair{small_, r} : sigmoid_pair{r, small_};
+}
+
+// The normal distribution's upper tail Q(w) = erfc(w / sqrt 2) / 2, w >= 0, and exp(-w^2 / 2): Q = t (c0 + c1 t + ...) exp(-w^2 / 2) with
+// t = 1 / (1 + p w).  The polynomials are fits of this file, minimax in the RELATIVE error over 0 <= w <= 14, beyond which both are 0: five powers
+// 5.2e-6 (2^-17), eight 4.3e-8 (2.9e-7 with the rounding of its terms).  An absolute bound would not do: gelu multiplies the tail by z.
+struct normal_tail { float q, e; };
+template <bool WIDE>
+__device__ __forceinline__ normal_tail tail_of(float w)
+{
+    if constexpr (WIDE) {
+#pragma clang fp contract(off)
+        constexpr float H = 0.721347511f, H_LO = 9.62981517e-09f;      // log2(e) / 2
+        const float sq = w * w, sq_lo = __builtin_fmaf(w, w, -sq), hi = sq * H;
+        const float e = exp2_neg(hi, __builtin_fmaf(sq_lo, H, __builtin_fmaf(sq, H_LO, __builtin_fmaf(sq, H, -hi))));
+        const float t = rcp_of(__builtin_fmaf(0.353553385f, w, 1.0f));
+        float p = -0.0295344628f;
+        constexpr float C[] = {0.142287403f, -0.243599832f, 0.139033467f, -0.0133127607f, 0.101343408f, 0.121551886f, 0.141187653f, 0.141043201f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p = __builtin_fmaf(p, t, C[i]);
+        return {p * t * e, e};
+    } else {
+        const float e = __builtin_amdgcn_exp2f(w * w * -0.721347520444481704f);
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.311126977f, w, 1.0f));
+        float p = -0.0730531216f;
+        constexpr float C[] = {0.175327092f, 0.0203646068f, 0.131793693f, 0.121284626f, 0.12428052f};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) p = __builtin_fmaf(p, t, C[i]);
+        return {p * t * e, e};
+    }
+}
+
 // Five activations in three forms, so that a kernel carries three pieces of code (their constants travel in epilogue_args):
 //   linear    z, or 0 below `floor` (0: relu; -inf: none)
-//   sigmoid   z sigmoid(z (p + q z^2)): silu, and gelu's tanh form, whose (1 + tanh u) / 2 is sigmoid(2 u); a, b = -p, -q times log2(e)
+//   sigmoid   z sigmoid(z (p + q z^2)): silu, and gelu's tanh form, whose (1 + tanh u) / 2 is sigmoid(2 u); a, b = -p, -q times log2(e), b = 0: silu
 //   erf       z Phi(z)
-// At -inf the factor is 0 and the limit is 0: the multiplicand is kept finite (a NaN comes back through the factor), and so is the square (b may be 0).
+// At -inf the factor is 0 and the limit is 0: the multiplicand is kept finite (a NaN stays, or comes back through the factor), and so is the square
+// (b may be 0).
 __device__ __forceinline__ float act_linear(float z, float floor) { return z < floor ? 0.0f : z; }
+template <bool WIDE>
 __device__ __forceinline__ float act_sigmoid(float z, float a, float b)
 {
+    if constexpr (WIDE) {
+        const float w = fabsf(z);
+        const float f = sigmoid_both(z < 0.0f, b == 0.0f ? silu_exponent(fminf(w, 200.0f)) : gelu_tanh_exponent(fminf(w, 20.0f))).s;
+        return (z < -FLT_MAX ? -FLT_MAX : z) * f;
+    }
     return fmaxf(z, -FLT_MAX) * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (a + b * fminf(z * z, 1e30f))));
 }
+template <bool WIDE>
 __device__ __forceinline__ float act_erf(float z)
 {
-    const float x = fabsf(z) * 0.707106781186547524f;
-    const float q = 0.5f * erfc_abs(x, exp_of(-x * x));
-    return fmaxf(z, -FLT_MAX) * (z < 0.0f ? q : 1.0f - q);
+    const float q = tail_of<WIDE>(fminf(fabsf(z), 20.0f)).q;
+    return (z < -FLT_MAX ? -FLT_MAX : z) * (z < 0.0f ? q : 1.0f - q);
 }
 
 // The derivative.  Beyond the limits it is 0 or 1 to the last bit of f32; inside them nothing overflows.
-template <int ACT>
+template <int ACT, bool WIDE>
 __device__ __forceinline__ float act_grad_of(float z)
 {
+    constexpr float P = 2.0f * GELU_C0, P3 = 3.0f * GELU_C1;
     if constexpr (ACT == MI355_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
     if constexpr (ACT == MI355_ACT_SILU) {
         z = limit(z, -120.0f, 120.0f);
+        if constexpr (WIDE) {
+            const sigmoid_pair f = sigmoid_both(z < 0.0f, silu_exponent(fminf(fabsf(z), 120.0f)));
+            return f.s * (1.0f + z * f.c);
+        }
         const float s = sigmoid_of(z);
         return s * (1.0f + z * (1.0f - s));
     }
     if constexpr (ACT == MI355_ACT_GELU_TANH) {
         z = limit(z, -20.0f, 20.0f);
-        const float s = sigmoid_of(2.0f * GELU_C0 * z * (1.0f + GELU_C1 * z * z));
-        return s + z * s * (1.0f - s) * (2.0f * GELU_C0) * (1.0f + 3.0f * GELU_C1 * z * z);
+        if constexpr (WIDE) {
+            const sigmoid_pair f = sigmoid_both(z < 0.0f, gelu_tanh_exponent(fminf(fabsf(z), 20.0f)));
+            return f.s * (1.0f + z * f.c * (P * (1.0f + P3 * z * z)));
+        }
+        const float s = sigmoid_of(P * z * (1.0f + GELU_C1 * z * z));
+        return s + z * s * (1.0f - s) * P * (1.0f + P3 * z * z);
     }
     if constexpr (ACT == MI355_ACT_GELU) {
         z = limit(z, -20.0f, 20.0f);
-        const float x = fabsf(z) * 0.707106781186547524f, ex = exp_of(-x * x);
-        const float q = 0.5f * erfc_abs(x, ex);
-        return (z < 0.0f ? q : 1.0f - q) + z * ex * 0.398942280401432678f;      // Phi(z) + z phi(z)
+        const normal_tail t = tail_of<WIDE>(fminf(fabsf(z), 20.0f));
+        return (z < 0.0f ? t.q : 1.0f - t.q) + z * t.e * 0.398942280401432678f;      // Phi(z) + z phi(z)
     }
     return 1.0f;
 }

@@ -482,7 +482,8 @@ int32_t mi355_gemm_scaled_select(mi355_ctx *ctx, const mi355_gemm_scaled_desc *d
  *                 were quantised by row (mi355_rms_norm) and by column, or by tensor, are multiplied back here.
  * Outputs must not overlap operands or each other (residual == C above excepted); an overlap that can be told from the descriptors is refused.
  * NaN and infinities follow the formula; an activation of -inf is its limit (0 for relu, gelu and silu).
- * The exponentials are v_exp_f32 (relative error below 2^-22 for |z| < 1), erf is Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7).
+ * An activation is within 2^-20 of its value for an F32 output and within 2^-15 for a 16-bit one before its rounding, the tails of gelu and silu
+ * included (16-bit: what is below 2^-118 may be 0).
  * Every kernel that mi355_gemm may take runs the epilogue on its accumulators, or in the fold of its K slices: scratch, capture windows and
  * the choice of kernel are mi355_gemm's (the persistent 256x256 forms are replaced by the same tile, one a workgroup). */
 enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_GELU = 2 /* z * Phi(z) */, MI355_ACT_GELU_TANH = 3 /* its tanh form */, MI355_ACT_SILU = 4 };

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from cubecl_amd import TensorHandle, ops
-from test_gpu_linear_ops import BF16, E4M3, E5M2, F32, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, raw_down, rng, rounded, up
+from cubecl_amd import _native as N
+from test_gpu_linear_ops import BF16, E4M3, E5M2, F32, FLOATS, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, raw_down, rng, rounded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +108,45 @@ def test_8_bit_rows_are_quotients(client, rows, cols, out_dt):
     ops.rms_norm(client, x, w, q, scales=s)
     want = (down(client, y).float() / down(client, s).float()[:, None]).to(TORCH[out_dt])
     assert torch.equal(raw_down(client, q), want.view(torch.uint8).reshape(-1))
+
+
+# ---- activations to their tails -----------------------------------------------------------------------------------------------------------
+# f32: exp2 1 ulp, its exponent in two pieces, the fit 4.3e-8 (2.9e-7 with its terms' rounding, evaluated in f32 over the whole range), three products
+# of half an ulp each: below 8e-7 < 2^-20 of the value; a subnormal exponential is 2^-149 off, times |z|.  16-bit outputs: the fit 5.2e-6, the
+# exponent |u| 2^-23 with |u| <= 88: below 2.4e-5 < 2^-15, then half a step of the type; what the instruction flushes is below 2^-118.
+def tails(dt):
+    z = torch.cat([torch.linspace(-104.0, 20.0, 2000), torch.linspace(-14.0, 6.0, 2000), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-4, -1e-4])]).to(TORCH[dt])
+    return z[: z.numel() // 8 * 8]
+
+
+def tail_tol(z, terms, dt):
+    return 2.0 ** -20 * terms + (z.abs() + 2) * 2.0 ** -148 if dt == F32 else 2.0 ** -15 * terms + 2.0 ** -118
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dt", FLOATS, ids=lambda d: d.name)
+@pytest.mark.parametrize("m,k,algo", [(1, 64, N.GEMM_ALGO_AUTO), (4, 64, N.GEMM_ALGO_GENERIC), (130, 64, N.GEMM_ALGO_AUTO), (130, 64, N.GEMM_ALGO_EDGE), (16, 8192, N.GEMM_ALGO_EDGE)])
+def test_activation_tails(client, act, dt, m, k, algo):
+    """Relative to the value, wherever the type has a number for it: on the tiles, element by element and in the fold of K slices."""
+    z = tails(dt)
+    out = empty(client, (m, z.numel()), dt)
+    ops.matmul_fused(client, up(client, torch.zeros(m, k).to(z.dtype)), up(client, torch.zeros(k, z.numel()).to(z.dtype)), out, bias=up(client, z), activation=act, algo=algo)
+    z = z.double().expand(m, -1)
+    ref = act64(act, z)[0]
+    close(down(client, out), ref, rounded(ref, tail_tol(z, ref.abs(), dt), dt) if dt != F32 else tail_tol(z, ref.abs(), dt))
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dt", FLOATS, ids=lambda d: d.name)
+def test_activation_gradient_tails(client, act, dt):
+    """The derivative is a sum of two terms that may cancel: its error relative to theirs, twice a value's (each is two factors).  An f32 sigmoid
+    below the normal numbers is a step of 2^-149 off (exponential and product half of one each), and the second term multiplies it by z u'(z): u' is 1
+    for silu and sqrt(8 / pi) (1 + 3 c z^2), c = 0.044715, up to 25 at z = -10.6, for gelu's tanh form."""
+    z = tails(dt)[None]
+    dz = empty(client, tuple(z.shape), dt)
+    ops.matmul_fused_backward(client, up(client, torch.ones_like(z)), up(client, z), dz, activation=act)
+    z = z.double()
+    y, ref = act64(act, z)
+    part = torch.where(z == 0, 0.5, y / torch.where(z == 0, 1.0, z))                # Phi(z), sigmoid(u)
+    slope = (8 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * z * z) if act == "gelu_tanh" else torch.ones_like(z)
+    close(down(client, dz), ref, rounded(ref, 2 * tail_tol(z * slope, part.abs() + (ref - part).abs(), dt), dt))

@@ -777,7 +777,7 @@ bool edge_wins(const mi355_gemm_desc &d, const void *a, const void *b, const voi
     return flops <= (d.dtype_ab != MI355_DTYPE_F32 && !d.trans_a && d.trans_b ? 40e9 : 8e9);
 }
 
-// mi355_gemm of a validated descriptor, with the epilogue `ep` where one is given
+// mi355_gemm of a validated descriptor, with the epilogue `ep` where one is given (it may have no parts)
 int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, const void *a, const void *b, void *c, const epilogue_args *ep)
 {
     mi355_gemm_desc d = desc;
@@ -785,6 +785,8 @@ int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, con
         return launch_gemm_edge(ctx, s, d, a, b, c, *ep);
     if (d.algo == MI355_GEMM_ALGO_EDGE)
         return fail(ctx, MI355_E_UNSUPPORTED, "mi355_gemm: the edge kernel belongs to mi355_gemm_fused and takes f32, bf16 and f16 operands with k > 0");
+    // nothing to do on the accumulators: the plain product on its own kernels, the persistent ones among them (the products of a gradient)
+    if (ep && !has_parts(*ep)) ep = nullptr;
     int32_t algo = d.algo == MI355_GEMM_ALGO_AUTO ? select_auto(d, a, b, c) : d.algo;
     if (d.algo == MI355_GEMM_ALGO_AUTO && algo == MI355_GEMM_ALGO_GENERIC) {
         mi355_gemm_desc nd;
@@ -810,8 +812,8 @@ int32_t run_gemm(mi355_ctx *ctx, hipStream_t s, const mi355_gemm_desc &desc, con
         }
     }
     // 8-bit operands, at most two 128 x 128 tiles a CU: two co-resident workgroups hide each other's epilogue where the square tile waits for its
-    // own (us, square / 128: 1777 x 4096 x 4096 with silu and residual 55.6 / 45.1, without 48.3 / 40.7, 2048 x 4096 x 4096 56.8 / 47.4; three tiles a
-    // CU the other way, 2560 x 4096 x 4096 57.3 / 79.6)
+    // own (us, square / 128: 1777 x 4096 x 4096 with silu and residual 55.6 / 45.1, 2048 x 4096 x 4096 56.8 / 47.4; three tiles a CU the other way,
+    // 2560 x 4096 x 4096 57.3 / 79.6; without parts the square tile's own stores, 41.3 for 1777 x 4096 x 4096)
     if (ep && d.algo == MI355_GEMM_ALGO_AUTO && algo == MI355_GEMM_ALGO_LP_256W4 && is_fp8(d.dtype_ab) && tiles_of(d, 128, 128) <= 2 * rule::CUS &&
         gemm_lp128_supports(d, a, b, c))
         algo = MI355_GEMM_ALGO_LP_128;

@@ -114,6 +114,10 @@ inline epilogue_args make_epilogue(const mi355_gemm_epilogue &ep, int32_t dtype_
     e.b = ep.activation == MI355_ACT_SILU ? 0.0f : -2.0f * GELU_C0 * GELU_C1 * LOG2E;
     return e;
 }
+inline bool has_parts(const epilogue_args &e)
+{
+    return e.p.bias || e.p.residual || e.p.pre || e.p.row_scale || e.p.col_scale || e.p.activation != MI355_ACT_NONE;
+}
 // the same for the part of the output that begins at (row, col)
 inline epilogue_args epilogue_at(epilogue_args e, int64_t row, int64_t col)
 {

@@ -485,7 +485,7 @@ int32_t mi355_gemm_scaled_select(mi355_ctx *ctx, const mi355_gemm_scaled_desc *d
  * An activation is within 2^-20 of its value for an F32 output and within 2^-15 for a 16-bit one before its rounding, the tails of gelu and silu
  * included (16-bit: what is below 2^-118 may be 0).
  * Every kernel that mi355_gemm may take runs the epilogue on its accumulators, or in the fold of its K slices: scratch, capture windows and
- * the choice of kernel are mi355_gemm's (the persistent 256x256 forms are replaced by the same tile, one a workgroup). */
+ * the choice of kernel are mi355_gemm's (with any part given, the persistent 256x256 forms are replaced by the same tile, one a workgroup). */
 enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_GELU = 2 /* z * Phi(z) */, MI355_ACT_GELU_TANH = 3 /* its tanh form */, MI355_ACT_SILU = 4 };
 typedef struct {
     const void *bias, *residual;

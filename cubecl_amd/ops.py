@@ -633,7 +633,9 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
         grad_lhs = grad_pre @ rhs^T                   grad_rhs = lhs^T @ grad_pre
 
     and the residual's gradient is grad_out itself.  Outputs that are not given are not computed; grad_pre (grad_out's shape and dtype, f32, bf16
-    or f16; may be grad_out or pre_activation itself) is needed for the products, which take it as it is stored; grad_bias sums it before its rounding.
+    or f16; may be grad_out or pre_activation itself) is needed for the products, which take it as it is stored: each of
+    their terms carries half a step of its type (bf16 2^-8, f16 2^-11 relative), as the products of stored gradients do.  grad_bias sums it before
+    its rounding.
     `pre_activation` may be None for activation "none".  grad_bias: [n] or [batch.., n], f32 or grad_out's dtype.  An operand that matmul_fused
     broadcast over the batch gets the sum over the batch."""
     what = "matmul_fused_backward"

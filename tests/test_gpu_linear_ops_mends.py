@@ -1,11 +1,13 @@
 """Calls of the operators around a linear layer that once gave a wrong result or read what was not theirs, on the MI355X, against their formulas in
 64 bits.  Helpers and tolerances are tests/test_gpu_linear_ops.py's unless a test says otherwise."""
+import ctypes as C
+
 import pytest
 import torch
 
 from cubecl_amd import TensorHandle, ops
 from cubecl_amd import _native as N
-from test_gpu_linear_ops import BF16, E4M3, E5M2, F32, FLOATS, TORCH, act64, act_tol, close, down, empty, grad_tol, rand, raw_down, rng, rounded, up
+from test_gpu_linear_ops import BF16, E4M3, E5M2, F32, FLOATS, TORCH, Step, act64, act_tol, close, down, empty, grad_tol, rand, raw_down, rng, rounded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +152,28 @@ def test_activation_gradient_tails(client, act, dt):
     part = torch.where(z == 0, 0.5, y / torch.where(z == 0, 1.0, z))                # Phi(z), sigmoid(u)
     slope = (8 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * z * z) if act == "gelu_tanh" else torch.ones_like(z)
     close(down(client, dz), ref, rounded(ref, 2 * tail_tol(z * slope, part.abs() + (ref - part).abs(), dt), dt))
+
+
+# ---- streams ----------------------------------------------------------------------------------------------------------------------------
+def test_steps_on_two_streams_write_what_they_should(client):
+    """Two programs at once on streams of their own, their outputs filled with 0xFF before each pass: work that was dropped, ended early or mixed up
+    with the other program's workspaces and scratch shows in every pass."""
+    steps = [Step(client, 90), Step(client, 91, rows=33, wide=512)]
+    want = []
+    for st in steps:
+        st.run(client)
+        want.append(st.bits(client))
+    lanes = [client.with_stream(1), client.with_stream(2)]
+    for i in range(4):
+        for st in steps:
+            for v in st.o.values():
+                client._s.check(client.lib.mi355_memset(client.ctx, client.on(v), C.c_void_p(v.device_ptr()), 0xFF, v.handle.size_in_used()))
+        client.sync()
+        for _ in range(2):
+            for st, lane in (zip(steps, lanes) if i % 2 else zip(steps[::-1], lanes)):
+                st.run(lane)
+        for lane in lanes:
+            lane.sync()
+        for st, w in zip(steps, want):
+            got = st.bits(client)
+            assert all(torch.equal(got[k], w[k]) for k in w), (i, [k for k in w if not torch.equal(got[k], w[k])])

@@ -700,6 +700,9 @@ def matmul_fused_backward(client: ComputeClient, grad_out: TensorHandle, pre_act
         entries = grad_bias.num_elems() // n if n else 1
         if entries not in (1, batch):
             raise ServerError(N.E_INVALID_ARGUMENT, f"{what}: grad_bias has {entries} entries for batch {batch}")
+        if grad_bias.num_elems() == 0:              # one bias an entry, and no entries: nothing to write
+            grad_bias = None
+    if grad_bias is not None:
         desc.dtype_bias, desc.batch_bias = int(grad_bias.dtype), int(entries == batch and batch > 1)
         client._s.check(client.lib.mi355_gemm_fused_grad_workspace_bytes(C.byref(desc), C.byref(need)))
         if need.value:

@@ -50,6 +50,15 @@ def test_gradients_of_shared_operands_over_an_empty_batch_are_written(client, mo
     assert done == [((4, 0), (0, 5), (4, 5), None), ((4, 5), (4, 5)), ((5, 0), (0, 6), (5, 6), None), ((5, 6), (5, 6))]
 
 
+def test_a_bias_gradient_of_no_entries_is_not_written(client):  # noqa: F811
+    """[0, n]: one bias for each of no entries holds nothing, unlike [n], which is the sum over none."""
+    ops.matmul_fused_backward(client, make(client, (0, 4, 6)), None, make(client, (0, 4, 6)), grad_bias=make(client, (0, 6)))
+    assert log(client)["fold"] == 0
+    ops.matmul_fused_backward(client, make(client, (0, 4, 6)), None, make(client, (0, 4, 6)), grad_bias=make(client, (6,)))
+    ops.matmul_fused_backward(client, make(client, (3, 0, 6)), None, make(client, (3, 0, 6)), grad_bias=make(client, (3, 6)))
+    assert log(client)["fold"] == 2
+
+
 # ---- launch limits ------------------------------------------------------------------------------------------------------------------
 GEOMETRY = r"""
 #include "../../cubecl_amd/csrc/linear_ops.hpp"

@@ -1,10 +1,10 @@
 // global_norm.hip -- mi355_global_norm and mi355_clip_by_global_norm: sqrt(sum of x^2) over a list of tensors, and the list scaled by
 // min(1, max_norm / norm).
 //
-// Roofline: HBM.  Clipping cannot start to write before the last element is read, so the list is read twice and written once (0.57 GB of bf16:
-// 86 us of reading and 211 of copying at this card's rates; measured 334 together).  Outputs are stored past the caches: 360 -> 334 us, since
-// the second reading finds more of the list in the 256 MiB Infinity Cache.  (Walking the list backwards in the second pass: 334.0 / 335.1,
-// not worth its code; 8 and 16 workgroups a CU instead of 4: 343 and 386.)
+// Roofline: HBM.  Clipping cannot start to write before the last element is read, so the list is read twice and written once (0.60 GB of bf16:
+// 90 us of reading and 217 of copying at this card's rates; measured 123 and 214, 337 together, 370 in place).  Outputs are stored past the caches:
+// 360 -> 334 us, since the second reading finds more of the list in the 256 MiB Infinity Cache.  (Walking the list backwards in the second pass:
+// 334.0 / 335.1, not worth its code; 8 and 16 workgroups a CU instead of 4: 343 and 386.)
 //   - The list travels in the kernel arguments (no device table to upload, nothing for a captured graph to find changed): up to FLAT_MAX
 //     contiguous tensors or ROWS_MAX pitched ones a launch.
 //   - A launch's tensors are cut into chunks of CHUNK elements, dealt to the workgroups in turn; a workgroup finds a chunk's tensor by

@@ -9,6 +9,7 @@
 #include <cstring>
 #include <deque>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <set>
 #include <string>
@@ -34,6 +35,17 @@ struct mi355_profile_slot {
 };
 
 namespace mi355 { struct memory_pool; }   // pool.cpp
+
+// Library scratch and arrival tickets belong to a stream, and a graph captured there carries their addresses to whichever stream it is
+// replayed on: two such graphs on two streams, or one beside the capture stream's own calls, would count on the same words at once.
+// All graphs of one capture stream share this record; a replay elsewhere waits for that stream's work so far and for the last replay
+// elsewhere (`last`), and the stream's own later work waits for it.  A replay on the capture stream itself costs nothing.
+struct mi355_replay_order {
+    hipStream_t stream = nullptr;         // the capture stream, NULL once it is destroyed (its work is finished by then)
+    hipEvent_t last = nullptr;
+    bool owed = false;                    // the stream is under capture and has yet to wait for `last` (end_capture)
+    ~mi355_replay_order() { if (last) hipEventDestroy(last); }
+};
 
 // One per DeviceId; the reference's HipServer + HipContext
 // (crates/cubecl-hip/src/compute/server.rs:151-161).
@@ -82,6 +94,8 @@ struct mi355_ctx {
     // it, ticket_retired = slots of destroyed streams still pinned
     std::set<uint32_t> capture_tickets, ticket_retired;
     std::map<uint32_t, int> ticket_refs;
+    // per capture stream: orders the replays on other streams of the graphs that carry its scratch or its tickets (runtime.cpp)
+    std::map<hipStream_t, std::shared_ptr<mi355_replay_order>> replay_orders;
     // library-owned device scratch per (stream, kind): split-K slabs, re-laid-out GEMM operands
     std::map<std::pair<hipStream_t, int>, std::pair<void *, size_t>> scratch;
     mi355::memory_pool *pool = nullptr;    // caching allocator behind mi355_pool_* (pool.cpp)

@@ -419,6 +419,10 @@ MI355_API int32_t mi355_stream_destroy(mi355_ctx *ctx, mi355_stream stream)
         else ctx->ticket_free.push_back(slot->second);
         ctx->ticket_slots.erase(slot);
     }
+    if (const auto order = ctx->replay_orders.find(s); order != ctx->replay_orders.end()) {
+        order->second->stream = nullptr;       // its graphs go on, ordered among themselves
+        ctx->replay_orders.erase(order);
+    }
     MI355_HIP(ctx, hipStreamDestroy(s));
     return MI355_OK;
 }
@@ -897,6 +901,7 @@ struct mi355_graph {
     std::set<void *> scratch;             // library scratch its nodes carry
     std::set<uint32_t> tickets;           // arrival-ticket slots its nodes carry
     std::set<hipStream_t> streams;        // streams it was replayed on (waited for before the executable dies)
+    std::shared_ptr<mi355_replay_order> order;   // NULL: its nodes carry neither scratch nor tickets
 };
 
 // A capture that fails pins nothing: slots handed out in its window go back to being ordinary -- and the slot of a stream that was
@@ -918,6 +923,9 @@ MI355_API int32_t mi355_graph_begin_capture(mi355_ctx *ctx, mi355_stream stream)
 {
     MI355_REQUIRE_CTX(ctx);
     if (ctx->capturing) return fail(ctx, MI355_E_INVALID_ARGUMENT, "begin_capture: a capture is already open on this context");
+    // no event of the stream can be recorded for another stream while the window is open: a replay elsewhere waits for this one
+    if (const auto order = ctx->replay_orders.find(stream_of(ctx, stream)); order != ctx->replay_orders.end())
+        MI355_HIP(ctx, hipEventRecord(order->second->last, stream_of(ctx, stream)));
     MI355_HIP(ctx, hipStreamBeginCapture(stream_of(ctx, stream), hipStreamCaptureModeThreadLocal));
     ctx->capturing = true;
     ctx->capture_stream = stream_of(ctx, stream);
@@ -933,6 +941,7 @@ MI355_API int32_t mi355_graph_end_capture(mi355_ctx *ctx, mi355_stream stream, m
     if (!out_graph) return fail(ctx, MI355_E_INVALID_ARGUMENT, "end_capture: out_graph is NULL");
     *out_graph = nullptr;
     if (!ctx->capturing) return fail(ctx, MI355_E_INVALID_ARGUMENT, "end_capture without begin_capture");
+    const hipStream_t captured = ctx->capture_stream;
     ctx->capturing = false;
     ctx->capture_stream = nullptr;
     ctx->captured_events.clear();
@@ -940,6 +949,13 @@ MI355_API int32_t mi355_graph_end_capture(mi355_ctx *ctx, mi355_stream stream, m
     ctx->capture_id = 0;
     hipGraph_t g = nullptr;
     hipError_t e = hipStreamEndCapture(stream_of(ctx, stream), &g);
+    if (const auto order = ctx->replay_orders.find(captured); order != ctx->replay_orders.end() && order->second->owed) {
+        order->second->owed = false;
+        if (const hipError_t w = hipStreamWaitEvent(captured, order->second->last, 0); w != hipSuccess) {
+            (void)hipGetLastError();
+            queue_error(ctx, MI355_E_EXECUTION, 0, 0, "end_capture: hipStreamWaitEvent: %s", hipGetErrorString(w));
+        }
+    }
     hipGraphExec_t x = nullptr;
     if (e != hipSuccess || !g) {
         (void)hipGetLastError();
@@ -949,7 +965,16 @@ MI355_API int32_t mi355_graph_end_capture(mi355_ctx *ctx, mi355_stream stream, m
         return fail(ctx, MI355_E_EXECUTION, "hipStreamEndCapture: %s (an operation in the window was not capturable: "
                     "run the sequence once before capturing so that library scratch exists)", hipGetErrorString(e));
     }
-    e = hipGraphInstantiate(&x, g, nullptr, nullptr, 0);
+    std::shared_ptr<mi355_replay_order> order;
+    if (!ctx->capture_scratch.empty() || !ctx->capture_tickets.empty()) {
+        std::shared_ptr<mi355_replay_order> &known = ctx->replay_orders[captured];
+        if (!known) known = std::make_shared<mi355_replay_order>();
+        known->stream = captured;
+        if (!known->last) e = hipEventCreateWithFlags(&known->last, hipEventDisableTiming);
+        order = known;
+        if (e != hipSuccess) ctx->replay_orders.erase(captured);
+    }
+    if (e == hipSuccess) e = hipGraphInstantiate(&x, g, nullptr, nullptr, 0);
     if (e != hipSuccess) {
         hipGraphDestroy(g);
         pool_release_graph(ctx, id);
@@ -959,7 +984,7 @@ MI355_API int32_t mi355_graph_end_capture(mi355_ctx *ctx, mi355_stream stream, m
     }
     // From here on the graph owns a pin on every pool block allocated or freed in its window (pool.cpp keeps them out of
     // the free lists under `id`) and on the library scratch its kernels were captured with.
-    mi355_graph *out = new mi355_graph{g, x, id, {}, {}, {}};
+    mi355_graph *out = new mi355_graph{g, x, id, {}, {}, {}, order};
     out->scratch.swap(ctx->capture_scratch);
     for (void *p : out->scratch) ++ctx->scratch_refs[p];
     out->tickets.swap(ctx->capture_tickets);
@@ -973,8 +998,21 @@ MI355_API int32_t mi355_graph_replay(mi355_ctx *ctx, mi355_stream stream, mi355_
 {
     MI355_REQUIRE_CTX(ctx);
     if (!graph) return fail(ctx, MI355_E_NOT_FOUND, "replay: unknown graph");
-    graph->streams.insert(stream_of(ctx, stream));
-    hipError_t e = hipGraphLaunch(graph->exec, stream_of(ctx, stream));
+    const hipStream_t s = stream_of(ctx, stream);
+    mi355_replay_order *order = graph->order && graph->order->stream != s ? graph->order.get() : nullptr;
+    const bool recorded = order && order->stream && !(ctx->capturing && ctx->capture_stream == order->stream);
+    hipError_t e = hipSuccess;
+    if (recorded) e = hipEventRecord(order->last, order->stream);      // that stream already waits for the replays elsewhere before it
+    if (order && e == hipSuccess) e = hipStreamWaitEvent(s, order->last, 0);
+    if (e == hipSuccess) {
+        graph->streams.insert(s);
+        e = hipGraphLaunch(graph->exec, s);
+        if (order && e == hipSuccess) {
+            e = hipEventRecord(order->last, s);
+            if (e == hipSuccess && recorded) e = hipStreamWaitEvent(order->stream, order->last, 0);
+            else if (e == hipSuccess && order->stream) order->owed = true;
+        }
+    }
     if (e != hipSuccess) {                       // fire-and-forget like launch: queued, reported by flush / sync
         (void)hipGetLastError();
         queue_error(ctx, MI355_E_LAUNCH, 0, 0, "hipGraphLaunch: %s", hipGetErrorString(e));

@@ -827,7 +827,11 @@ int32_t mi355_sum_argmax_exchange(mi355_ctx *ctx, mi355_comm *comm, mi355_stream
  * stream between begin and end into a hipGraph and replays it with one launch -- for launch-bound
  * sequences (an empty kernel costs ~2.7 us of host time here).  Run the sequence once before capturing
  * (graph_prepare + warm-up in the reference, base.rs:453-470) so that lazily created library scratch
- * exists; nothing the library enqueues synchronises the host or allocates after that. */
+ * exists; nothing the library enqueues synchronises the host or allocates after that.
+ * A graph may be replayed on any stream of its context.  Where its kernels use the scratch or the tickets
+ * that the library keeps for the capture stream (K slices, re-laid-out operands, reductions), a replay on
+ * another stream takes its turn with the capture stream's work and with the other replays of that stream's
+ * graphs; the order of the program's own tensors is the program's affair, as between any two streams. */
 typedef struct mi355_graph mi355_graph;
 int32_t mi355_graph_begin_capture(mi355_ctx *ctx, mi355_stream stream);
 int32_t mi355_graph_end_capture(mi355_ctx *ctx, mi355_stream stream, mi355_graph **out_graph);

@@ -7,6 +7,7 @@
 #include <mutex>
 #include <set>
 #include <sys/mman.h>
+#include <tuple>
 
 struct fake_hip_stream { uint64_t submitted = 0, completed = 0; };
 struct fake_hip_event { fake_hip_stream *stream = nullptr; uint64_t seq = 0; };
@@ -18,6 +19,7 @@ struct fake_state {
     uint64_t mallocs = 0, frees = 0, bad_frees = 0, event_creates = 0, event_destroys = 0, event_queries = 0, device_syncs = 0;
     std::set<fake_hip_stream *> streams;
     std::set<fake_hip_event *> events;
+    std::vector<std::tuple<char, const void *, const void *>> order;   // ('r' record | 'w' wait | 'g' graph launch, stream, event or graph) as queued
 } g;
 // One lock around the whole fake: the real runtime is thread-safe and the library is driven from one thread per device
 // (tests/test_comm_cpu.py THREADED: four contexts created, used and destroyed concurrently).
@@ -89,6 +91,7 @@ hipError_t hipEventRecord(hipEvent_t event, hipStream_t stream)
     if (!event || !stream) return hipErrorInvalidValue;
     event->stream = stream;
     event->seq = ++stream->submitted;          // the record itself is a piece of work on the stream
+    g.order.emplace_back('r', stream, event);
     return hipSuccess;
 }
 
@@ -249,7 +252,7 @@ hipError_t hipStreamSynchronize(hipStream_t s)
     r.fail_next_sync = hipSuccess;
     return e;
 }
-hipError_t hipStreamWaitEvent(hipStream_t s, hipEvent_t, unsigned) { ++r.stream_waits; r.last_wait_stream = s; return hipSuccess; }
+hipError_t hipStreamWaitEvent(hipStream_t s, hipEvent_t e, unsigned) { LOCKED; ++r.stream_waits; r.last_wait_stream = s; g.order.emplace_back('w', s, e); return hipSuccess; }
 hipError_t hipEventCreate(hipEvent_t *e) { return hipEventCreateWithFlags(e, 0); }
 hipError_t hipEventSynchronize(hipEvent_t e) { LOCKED; if (e && e->stream) e->stream->completed = e->stream->submitted; return hipSuccess; }
 hipError_t hipEventElapsedTime(float *ms, hipEvent_t, hipEvent_t) { *ms = 1.5f; return hipSuccess; }
@@ -301,7 +304,7 @@ hipError_t hipStreamEndCapture(hipStream_t, hipGraph_t *graph)
     return hipSuccess;
 }
 hipError_t hipGraphInstantiate(hipGraphExec_t *x, hipGraph_t graph, void *, char *, size_t) { *x = new fake_hip_graph_exec{graph->nodes}; return hipSuccess; }
-hipError_t hipGraphLaunch(hipGraphExec_t x, hipStream_t st) { r.graph_launches += 1; r.launches += (uint64_t)x->nodes; work(st); return hipSuccess; }
+hipError_t hipGraphLaunch(hipGraphExec_t x, hipStream_t st) { r.graph_launches += 1; r.launches += (uint64_t)x->nodes; work(st); { LOCKED; g.order.emplace_back('g', st, x); } return hipSuccess; }
 hipError_t hipGraphExecDestroy(hipGraphExec_t x) { delete x; return hipSuccess; }
 hipError_t hipGraphDestroy(hipGraph_t graph) { delete graph; return hipSuccess; }
 }  // extern "C"
@@ -323,6 +326,19 @@ TEST_API void faketest_stream_log(uint64_t out[4])
 {
     out[0] = r.stream_syncs; out[1] = r.stream_waits;
     out[2] = reinterpret_cast<uintptr_t>(r.last_wait_stream); out[3] = reinterpret_cast<uintptr_t>(r.last_sync_stream);
+}
+// what was queued since the last call: up to `room` entries {kind, stream, event or graph}; returns their number and forgets them
+TEST_API uint64_t faketest_queue_order(uint64_t *out, uint64_t room)
+{
+    LOCKED;
+    const uint64_t n = g.order.size() < room ? g.order.size() : room;
+    for (uint64_t i = 0; i < n; ++i) {
+        out[3 * i] = (uint64_t)std::get<0>(g.order[i]);
+        out[3 * i + 1] = reinterpret_cast<uintptr_t>(std::get<1>(g.order[i]));
+        out[3 * i + 2] = reinterpret_cast<uintptr_t>(std::get<2>(g.order[i]));
+    }
+    g.order.clear();
+    return n;
 }
 TEST_API void faketest_fail_end_capture(int32_t error) { r.fail_next_end_capture = (hipError_t)error; }
 #ifdef FAKE_WITH_RUNTIME

@@ -177,3 +177,35 @@ def test_steps_on_two_streams_write_what_they_should(client):
         for st, w in zip(steps, want):
             got = st.bits(client)
             assert all(torch.equal(got[k], w[k]) for k in w), (i, [k for k in w if not torch.equal(got[k], w[k])])
+
+
+def test_a_graph_of_k_slices_replayed_on_another_stream_beside_eager_calls(client):
+    """The slices' partial sums lie in scratch of the stream that the graph was captured on: replays on two other streams and that stream's own calls
+    of other operands, all queued at once, give what each gives alone."""
+    m, n, k = 1024, 512, 8192
+    g = rng(92)
+    w = up(client, rand(g, k, n, dt=BF16, scale=k ** -0.5))
+    rows = [up(client, rand(g, m, k, dt=BF16)) for _ in range(3)]
+    outs = [empty(client, (m, n), BF16) for _ in rows]
+    call = lambda i: ops.matmul_fused(client, rows[i], w, outs[i], activation="silu")
+    want = []
+    for i in range(3):
+        call(i)
+        want.append(raw_down(client, outs[i]))
+    lanes = [client.with_stream(1), client.with_stream(2)]
+    graphs = [client.capture(lambda i=i: call(i)) for i in range(2)]
+    try:
+        for _ in range(4):
+            for v in outs:
+                client._s.check(client.lib.mi355_memset(client.ctx, client.on(v), C.c_void_p(v.device_ptr()), 0xFF, m * n * 2))
+            client.sync()
+            for _ in range(6):
+                lanes[0].replay(graphs[0])
+                call(2)
+                lanes[1].replay(graphs[1])
+            for lane in (*lanes, client):
+                lane.sync()
+            assert all(torch.equal(raw_down(client, v), x) for v, x in zip(outs, want))
+    finally:
+        for graph in graphs:
+            client.graph_destroy(graph)
